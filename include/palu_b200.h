@@ -276,6 +276,43 @@ int palu_pack_cs_table(const void* cs_tab, int64_t ld, int32_t in_dtype, void* c
                        palu_stream_t stream);
 
 /*
+ * Causal attention of packed prompts. No counterpart in the reference, whose prefill runs the stock attention on one
+ * user's padded prompt (palu_tt/attention.py:382-516).
+ *
+ * Sequence s of a batch has q_lens[s] query positions and k_lens[s] keys, packed one sequence after another; its last
+ * query is aligned with its last key, so the query at offset i sees keys 0 .. i + k_lens[s] - q_lens[s] (a prompt:
+ * equal lengths; a prompt chunk behind a cached prefix: more keys than queries). A query that sees no key gives 0.
+ * Query head h attends KV head h / (n_q_heads / n_kv_heads); at most 128 query heads share a KV head.
+ *
+ * palu_plan_prefill lays the batch's work out for n_ctas thread blocks (0: one per SM of the current device) into
+ * `buf` (host memory of at least plan->bytes bytes; PALU_ERR_WORKSPACE if it is smaller, with plan->bytes set; NULL:
+ * sizes only). The caller copies the buffer to the device, 16-byte aligned, where palu_prefill_attn and
+ * palu_rebuild_kv read it: one plan serves every layer of a forward pass. Its first 4 bytes are a status word
+ * (palu_read_status). `rows` (NULL: 0, 1, ...): the cache row of each sequence, for palu_rebuild_kv.
+ */
+typedef struct palu_prefill_plan {
+  int64_t bytes, q_tokens, k_tokens;
+  int64_t off_start, off_pieces, off_merges, off_tiles; /* of the buffer's parts */
+  int32_t n_seq, n_q_heads, n_kv_heads, pos_per_chain;
+  int32_t n_ctas, n_pieces, n_merges, n_slots, n_tiles;
+} palu_prefill_plan;
+int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_t* rows, int32_t n_seq, int32_t n_q_heads,
+                      int32_t n_kv_heads, int32_t n_ctas, void* buf, size_t buf_bytes, palu_prefill_plan* plan);
+
+/*
+ * q [q_tokens][n_q_heads][128], k [k_tokens][n_kv_heads][128], v [k_tokens][n_kv_heads][d_v], bf16, with token and
+ * head strides in elements (multiples of 8; the last dimension is contiguous; 16-byte aligned); out
+ * [q_tokens][n_q_heads][d_v] bf16, contiguous. d_v a multiple of 16 in [16, 128]. scale > 0. plan_data: the plan's
+ * buffer on the device. workspace: palu_prefill_workspace_bytes(plan, d_v) bytes (0 for most plans; the partial
+ * results of work that was split along the keys), not shared by calls that overlap in time. A bounded device wait that
+ * expires sets the plan's status word, and the rows that it kept from being computed are NaN.
+ */
+size_t palu_prefill_workspace_bytes(const palu_prefill_plan* plan, int32_t d_v);
+int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                      const void* v, int64_t v_tok, int64_t v_head, void* out, int32_t d_v, const palu_prefill_plan* plan,
+                      void* plan_data, void* workspace, size_t workspace_bytes, float scale, palu_stream_t stream);
+
+/*
  * Select the decode kernel family for subsequent calls in this process (PALU_KERNEL_AUTO by default:
  * the tcgen05 kernel where its envelope covers the shapes, else the mma.sync kernel). No reference
  * counterpart (the Tensix op has one program); used to benchmark the legacy path against the product.

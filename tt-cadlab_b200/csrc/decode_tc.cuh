@@ -279,7 +279,7 @@ PALU_DEVINL unsigned long long globaltimer() {
 // already gave up. The polling loop is one out-of-line function: inlined at each of the ~20 wait sites it
 // grew the kernel body past what the instruction cache serves well (no_instruction stalls), and the op
 // measured 2-4 % faster on B200 with one shared copy.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status,
                                             unsigned long long limit_ns) {
   const unsigned long long t0 = globaltimer();
   for (;;) {

@@ -11,44 +11,15 @@
 #include <string>
 
 #include "../../include/palu_b200.h"
+#include "abi_common.h"
 #include "append.cuh"
 #include "combine.cuh"
 #include "decode_mma.cuh"
 #include "decode_tc.cuh"
 
+using namespace palu::abi;
+
 namespace {
-
-thread_local std::string g_err;
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_err = buf;
-  return code;
-}
-
-int cuda_check(const char* where) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(PALU_ERR_CUDA, "%s: %s", where, cudaGetErrorString(e));
-  return PALU_OK;
-}
-
-// SM count of the current device, cached per device. Several host threads may race on the first lookup;
-// each stores the same value, and the atomics make those stores and the loads well defined.
-int device_sms() {
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int n = cache[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    cache[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
-}
 
 int rep_of(const palu_decode_dims* d) { return d->n_q_heads / d->n_kv_heads; }
 
@@ -119,10 +90,6 @@ size_t ws_bytes(const palu_decode_dims* d, int splits) {
 int g_kernel_choice = PALU_KERNEL_AUTO;
 // RoPE form of this host thread's decode calls (palu_set_rope_mode).
 thread_local int g_rope_mode = PALU_ROPE_ABSOLUTE;
-// Timeout-path test hook (palu_set_wait_limit): the bound on every device wait, and the V-starve switch.
-std::atomic<unsigned long long> g_wait_ns{palu::tc::kWaitNs};
-std::atomic<int> g_starve_v{0};
-
 // Latents up to 128 wide run two pipelines per CTA; up to 256 wide, one (tc_pipes).
 bool tc_supported(const palu_decode_dims* d, bool recon) {
   return recon && d->r_k <= 256 && d->r_v <= 256 && rep_of(d) <= 4;
@@ -158,37 +125,6 @@ size_t ws_tc_bytes(const palu_decode_dims* d, int ctas) {
 
 int splits_for(const palu_decode_dims* d, bool recon) {
   return use_tc(d, recon) ? choose_splits_tc(d) : choose_splits(d);
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// The driver's cuTensorMapEncodeTiled, looked up once. A function-local static is initialised exactly once
-// even when several host threads make their first call at the same time.
-EncodeTiledFn encode_fn() {
-  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      return reinterpret_cast<EncodeTiledFn>(ptr);
-    return nullptr;
-  }();
-  return fn;
-}
-
-int encode(CUtensorMap* m, CUtensorMapDataType dt, int rank, const void* base, const cuuint64_t* dims,
-           const cuuint64_t* strides, const cuuint32_t* box, const char* what,
-           CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return fail(PALU_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = fn(m, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(PALU_ERR_INVALID, "tensor map for %s rejected (CUresult %d)", what, (int)r);
-  return PALU_OK;
 }
 
 // Page-table fields of the kernel parameters (all zero for contiguous caches).

@@ -1,0 +1,669 @@
+// Causal attention of packed prompts on the 5th-generation tensor cores (tcgen05 + TMEM + TMA).
+//
+// Sequence s has q_len query positions and k_len keys, its last query aligned with its last key: the query at
+// offset i sees the keys 0 .. i + k_len - q_len. With x_ij = scale q_i . k_j,
+//   o_i = sum_j exp(x_ij - m_i) v_j / l_i,   l_i = sum_j exp(x_ij - m_i),
+// in one pass over the keys with a running reference m_i and sum l_i (fp32); the exponentials are rounded to bf16
+// (half a step, 2^-9 relative) as the A operand of the second product, the two products accumulate in fp32.
+//
+// A work item is (sequence, query tile, KV head): two chains of 128 rows, where a chain's row is one (position, query
+// head of the KV head's group) pair, positions outermost, so that the heads that share K and V share their tiles and
+// a chain of rep heads per KV head covers 128 / rep positions (little masked work on the diagonal, and a prompt of
+// one token still fills rep rows). Items, or pieces of items along the keys, are laid out per CTA by the host's plan;
+// CTAs are persistent. A piece that is not a whole item writes a partial record (O, m, l) that the merge joins.
+// Per key tile t of 128 keys and chain c:
+//   MMA      S_c[128 x 128] (f32, TMEM) = Q_c (smem) x K_t^T (smem), 8 steps of K = 16
+//   softmax  one thread per row: row maximum, exp2, P_c (bf16) -> TMEM; O_c is rescaled only when a row's maximum
+//            outgrew its reference by more than 2^8 (any reference within that keeps P and l in range; the final
+//            division cancels it)
+//   MMA      O_c[128 x d_v] (f32, TMEM) += P_c (TMEM) x V_t (smem, MN-major: as TMA wrote it)
+// The chains run half a period apart: while the tensor cores work on one chain's PV and next S, the other chain's
+// softmax warps exponentiate. Values at most 64 wide leave TMEM columns for P of its own; wider ones write P over S.
+//
+// Masked places hold anything. Scores behind a row's last visible key are replaced, never added to. V rows behind the
+// item's last visible key are zeroed in shared memory before the product, and non-finite values in the V rows that
+// only some rows of the item see are zeroed too and added back, in the epilogue, to exactly the rows that see them
+// (0 * NaN in the tensor core would reach the others). A tile's V is checked only where the mask cuts it.
+//
+// Warps: 0..3 softmax of chain 0, 4..7 of chain 1, 8 TMA producer, 9 MMA issuer, 10 and 11 check V. Every wait is
+// bounded; on expiry the CTA records a status code, all roles stop, copies and MMAs in flight are drained, TMEM is
+// freed and the rows not yet written get NaN.
+#pragma once
+#include "decode_tc.cuh"
+
+namespace palu {
+namespace pf {
+
+using namespace palu::tc;
+
+constexpr int kPfThreads = 384;
+constexpr int kRows = 128;      // rows of a chain
+constexpr int kKeys = 128;      // keys of a tile
+constexpr int kQBytes = 2 * kBox, kKBytes = 2 * kBox;
+constexpr float kRescale = 8.f; // log2 of how far a row's maximum may outgrow its reference
+
+// One work piece: key tiles [t0, t1) of one (query tile, KV head).
+struct PfPiece {
+  int32_t q0;    // first packed query position
+  int32_t npos;  // query positions of the item (1 .. 2 * ppt)
+  int32_t vis0;  // keys that the first position sees (may be <= 0)
+  int32_t k0;    // packed index of the sequence's first key
+  int32_t kvh;
+  int32_t t0, t1;
+  int32_t slot;  // -1: the whole item; else the index of its partial record
+};
+// One cut item: its records are slots slot0 .. slot0 + n - 1.
+struct PfMerge {
+  int32_t q0, npos, vis0, kvh, slot0, n;
+};
+
+struct PfParams {
+  const PfPiece* pieces;
+  const int32_t* cta_start;  // [gridDim.x + 1]
+  __nv_bfloat16* out;        // [T][n_q][d_v]
+  float* ws_o;               // [slots][256][d_v]
+  float* ws_ml;              // [slots][256][2]
+  int* status;
+  const __nv_bfloat16* v;    // [Tk][n_kv][d_v] with the strides below (elements)
+  int64_t v_tok, v_head;
+  int n_q, rep, ppt, dv;
+  float sl2;                 // scale * log2(e)
+  unsigned long long wait_ns;
+  int starve;                // test of the timeout path: the producer loads no V
+};
+
+template <bool ALIAS>
+struct PfLayout {
+  static constexpr int NS_K = 3, NS_V = ALIAS ? 2 : 3;
+  static constexpr int V_BYTES = ALIAS ? 2 * kBox : kBox;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + 2 * kQBytes;
+  static constexpr int OFF_V = OFF_K + NS_K * kKBytes;
+  static constexpr int OFF_MISC = OFF_V + NS_V * V_BYTES;
+  static constexpr int TOTAL = OFF_MISC + 512 + 1024;
+  // TMEM columns
+  static constexpr uint32_t S = 0;                       // + 128 c
+  static constexpr uint32_t P = ALIAS ? 0 : 256;         // + P_STEP c
+  static constexpr uint32_t P_STEP = ALIAS ? 128 : 64;
+  static constexpr uint32_t O = ALIAS ? 256 : 384;       // + O_STEP c
+  static constexpr uint32_t O_STEP = ALIAS ? 128 : 64;
+  static_assert(TOTAL <= kSmemBudget, "shared memory budget");
+};
+
+// The tiles that chain c of a piece works on: t0 .. t0 + n - 1.
+struct PfChains {
+  int n[2];
+  int vis_first[2];  // keys that the chain's first position sees
+  int vis_max;       // keys that the item's last position sees
+  int nt;            // tiles of the piece
+  bool active[2];
+};
+PALU_DEVINL PfChains chains_of(const PfPiece& w, int ppt) {
+  PfChains s;
+  s.vis_max = w.vis0 + w.npos - 1;
+  s.nt = 0;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    s.active[c] = w.npos > c * ppt;
+    s.vis_first[c] = w.vis0 + c * ppt;
+    const int last = w.vis0 + min(w.npos, (c + 1) * ppt) - 1;  // keys that the chain's last position sees
+    const int tiles = s.active[c] && last > 0 ? (last + kKeys - 1) / kKeys : 0;
+    s.n[c] = max(0, min(w.t1, tiles) - w.t0);
+    s.nt = max(s.nt, s.n[c]);
+  }
+  return s;
+}
+// Whether some row of the item does not see every key of tile t.
+PALU_DEVINL bool tile_cut(const PfPiece& w, int t) { return (t + 1) * kKeys > w.vis0; }
+
+PALU_DEVINL float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+PALU_DEVINL uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+PALU_DEVINL void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+PALU_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+PALU_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+PALU_DEVINL void touch16(uint32_t* r) {  // a use of r that stays behind the volatile wait before it
+  asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+PALU_DEVINL void tmem_ld32p(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+PALU_DEVINL void tmem_st32p(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// Nonzero when one of the two bf16 in w is an infinity or a NaN (exponent all ones).
+PALU_DEVINL uint32_t nonfinite_bf16x2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+
+template <bool ALIAS>
+__global__ void __launch_bounds__(kPfThreads, 1)
+    palu_prefill_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v, const PfParams p) {
+  using Lay = PfLayout<ALIAS>;
+  constexpr int NS_K = Lay::NS_K, NS_V = Lay::NS_V;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w0 = p.cta_start[blockIdx.x], w1 = p.cta_start[blockIdx.x + 1];
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::OFF_MISC);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  // QF / QE: Q of chain c landed / free. KF / KE, VF / VE: ring slots. VC: the V tile of a cut tile has landed and is to
+  // be checked (by count of cut tiles, four in turn: more than the V ring holds); the checkers' two arrivals, instead of
+  // the copy's own, then complete VF, so a checker that looks at some tiles only never loses count of a phase. SF: S_c written. SR: S_c read (P of its own only). PF: P_c written. OD: PV_c done.
+  // OE: O_c read by the epilogue.
+  constexpr int B_QF = 0, B_QE = 2, B_KF = 4, B_KE = B_KF + NS_K, B_VF = B_KE + NS_K, B_VE = B_VF + NS_V,
+                B_VC = B_VE + NS_V, B_SF = B_VC + 4, B_SR = B_SF + 2, B_PF = B_SR + 2, B_OD = B_PF + 2, B_OE = B_OD + 2,
+                B_DRAIN = B_OE + 2, B_COUNT = B_DRAIN + 1;
+  static_assert(B_COUNT * 8 + 64 <= 512, "misc area");
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  volatile int* s_bad = reinterpret_cast<volatile int*>(s_tmem + 2);  // [4]: 1 + index of the last piece with non-finite V
+
+  auto wait = [&](uint32_t b, uint32_t ph) -> bool { return mbar_wait(b, ph, s_abort, p.status, p.wait_ns); };
+  auto wait_all = [&](uint32_t b, uint32_t ph) -> bool {
+    if (__all_sync(0xffffffffu, mbar_try(b, ph))) return true;
+    return __all_sync(0xffffffffu, mbar_wait_slow(b, ph, s_abort, p.status, p.wait_ns)) != 0;
+  };
+
+  // the same, inlined: the softmax warps run on more registers than the launch gave them, where no call compiles
+  auto wait_all_inline = [&](uint32_t b, uint32_t ph) -> bool {
+    bool done = mbar_try(b, ph);
+    if (!done) {
+      const unsigned long long t0 = globaltimer();
+      while (!(done = mbar_try(b, ph))) {
+        if (*s_abort) break;
+        if (globaltimer() - t0 > p.wait_ns) {
+          *s_abort = 1;
+          atomicExch(p.status, kStatusTimeout);
+          break;
+        }
+      }
+    }
+    return __all_sync(0xffffffffu, done) != 0;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int c = 0; c < 2; ++c) {
+      mbar_init(bar(B_QF + c), 1);
+      mbar_init(bar(B_QE + c), 1);
+      mbar_init(bar(B_SF + c), 1);
+      mbar_init(bar(B_SR + c), 4);
+      mbar_init(bar(B_PF + c), 4);
+      mbar_init(bar(B_OD + c), 1);
+      mbar_init(bar(B_OE + c), 4);
+    }
+    for (int s = 0; s < NS_K; ++s) {
+      mbar_init(bar(B_KF + s), 1);
+      mbar_init(bar(B_KE + s), 2);
+    }
+    for (int s = 0; s < NS_V; ++s) {
+      mbar_init(bar(B_VF + s), 2);
+      mbar_init(bar(B_VE + s), 2);
+    }
+    for (int s = 0; s < 4; ++s) mbar_init(bar(B_VC + s), 1);
+    mbar_init(bar(B_DRAIN), 1);
+    *s_abort = 0;
+    s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+    if (warp == 8 && lane == 0) {
+      // ============================== TMA producer ==============================
+      tma_prefetch_map(&tm_q);
+      tma_prefetch_map(&tm_k);
+      tma_prefetch_map(&tm_v);
+      const uint32_t q_bytes = (uint32_t)p.rep * p.ppt * 256;
+      const int vbox = (p.dv + 63) >> 6;
+      int nq[2] = {0, 0}, nk = 0, nv = 0, cut = 0;
+      uint32_t history = 0;  // which of the last V tiles were cut
+      bool ok = true;
+      auto load_k = [&](const PfPiece& w, int t) -> bool {
+        const int s = nk % NS_K, u = nk / NS_K;
+        if (u >= 1 && !wait(bar(B_KE + s), (u - 1) & 1)) return false;
+        mbar_expect_tx(bar(B_KF + s), kKBytes);
+        for (int b = 0; b < 2; ++b)
+          tma_load_3d(sbase + Lay::OFF_K + s * kKBytes + b * kBox, &tm_k, bar(B_KF + s), b * 64, w.kvh, w.k0 + t * kKeys);
+        ++nk;
+        return true;
+      };
+      for (int i = w0; ok && i < w1; ++i) {
+        const PfPiece w = p.pieces[i];
+        const PfChains ch = chains_of(w, p.ppt);
+        for (int c = 0; ok && c < 2; ++c) {
+          if (ch.n[c] == 0) continue;
+          if (nq[c] >= 1 && !(ok = wait(bar(B_QE + c), (nq[c] - 1) & 1))) break;
+          mbar_expect_tx(bar(B_QF + c), q_bytes);
+          for (int b = 0; b < 2; ++b)
+            tma_load_3d(sbase + Lay::OFF_Q + c * kQBytes + b * kBox, &tm_q, bar(B_QF + c), b * 64, w.kvh * p.rep,
+                        w.q0 + c * p.ppt);
+          ++nq[c];
+          if (c == 0 && ch.nt > 0) ok = load_k(w, w.t0);
+        }
+        if (ok && ch.n[0] == 0 && ch.nt > 0) ok = load_k(w, w.t0);
+        for (int j = 0; ok && j < ch.nt; ++j) {
+          if (j + 1 < ch.nt && !(ok = load_k(w, w.t0 + j + 1))) break;
+          const int s = nv % NS_V, u = nv / NS_V;
+          if (u >= 1 && !(ok = wait(bar(B_VE + s), (u - 1) & 1))) break;
+          if (p.starve) continue;
+          const bool is_cut = tile_cut(w, w.t0 + j);
+          const uint32_t full = is_cut ? bar(B_VC + (cut & 3)) : bar(B_VF + s);
+          mbar_expect_tx(full, vbox * kBox);
+          for (int b = 0; b < vbox; ++b)
+            tma_load_3d(sbase + Lay::OFF_V + s * Lay::V_BYTES + b * kBox, &tm_v, full, b * 64, w.kvh,
+                        w.k0 + (w.t0 + j) * kKeys);
+          if (!is_cut) mbar_arrive(full);
+          cut += is_cut;
+          history = history << 1 | (uint32_t)is_cut;
+          ++nv;
+        }
+      }
+      if (*s_abort) {  // let every copy already issued land before the CTA can exit
+        for (int c = 0; c < 2; ++c)
+          if (nq[c] > 0) mbar_drain(bar(B_QF + c), (nq[c] - 1) & 1);
+        for (int n = max(0, nk - NS_K); n < nk; ++n) mbar_drain(bar(B_KF + n % NS_K), (n / NS_K) & 1);
+        for (int n = nv - 1; n >= max(0, nv - NS_V); --n, history >>= 1) {
+          if (history & 1) {
+            --cut;
+            mbar_drain(bar(B_VC + (cut & 3)), (cut >> 2) & 1);
+          } else {
+            mbar_drain(bar(B_VF + n % NS_V), (n / NS_V) & 1);
+          }
+        }
+      }
+    } else if (warp == 9 && lane == 0) {
+      // ============================== MMA issuer ==============================
+      // For each tile, chain 0 then chain 1: PV_c of the tile, then the chain's next S (the next piece's first one
+      // included), so that the chains' turns at the tensor cores alternate.
+      const uint32_t ID_QK = idesc_f16(kKeys, 1, false, false), ID_PV = idesc_f16(p.dv, 1, false, true);
+      int ns[2] = {0, 0}, np[2] = {0, 0}, nq[2] = {0, 0}, no[2] = {0, 0};  // S, PV, Q loads and pieces per chain so far
+      int kb = 0;                  // ring index of the piece's first tile
+      int ahead[2] = {-1, -1};     // the piece whose first S the chain has issued already
+      bool ok = true;
+      auto issue_s = [&](int c, int n, bool first, bool last) -> bool {  // n: ring index of the K tile
+        if (first && !wait(bar(B_QF + c), nq[c]++ & 1)) return false;
+        if (!ALIAS && ns[c] >= 1 && !wait(bar(B_SR + c), (ns[c] - 1) & 1)) return false;
+        if (!wait(bar(B_KF + n % NS_K), (n / NS_K) & 1)) return false;
+        fence_after();
+        const uint32_t sK = sbase + Lay::OFF_K + (n % NS_K) * kKBytes, sQ = sbase + Lay::OFF_Q + c * kQBytes;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          mma_ss(tmem + Lay::S + 128 * c, sdesc(sQ + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024),
+                 sdesc(sK + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024), ID_QK, kk > 0);
+        mma_commit(bar(B_SF + c));
+        mma_commit(bar(B_KE + n % NS_K));
+        if (last) mma_commit(bar(B_QE + c));
+        ++ns[c];
+        return true;
+      };
+      for (int i = w0; ok && i < w1; ++i) {
+        const PfPiece w = p.pieces[i];
+        const PfChains ch = chains_of(w, p.ppt);
+        PfChains nx;
+        nx.n[0] = nx.n[1] = nx.nt = 0;
+        if (i + 1 < w1) nx = chains_of(p.pieces[i + 1], p.ppt);
+        for (int c = 0; ok && c < 2; ++c) {
+          if (ch.n[c] > 0) {
+            if (ahead[c] != i) ok = issue_s(c, kb, true, ch.n[c] == 1);
+          } else if (ch.nt > 0) {
+            mma_commit(bar(B_KE + kb % NS_K));
+          }
+        }
+        for (int j = 0; ok && j < ch.nt; ++j) {
+          const int n = kb + j, sv = n % NS_V;
+          if (!(ok = wait(bar(B_VF + sv), (n / NS_V) & 1))) break;
+          const uint32_t sV = sbase + Lay::OFF_V + sv * Lay::V_BYTES;
+          for (int c = 0; ok && c < 2; ++c) {
+            if (j >= ch.n[c]) {  // this chain sees nothing of the tile
+              mma_commit(bar(B_VE + sv));
+              if (j + 1 < ch.nt) mma_commit(bar(B_KE + (n + 1) % NS_K));
+              continue;
+            }
+            if (!(ok = wait(bar(B_PF + c), np[c] & 1))) break;
+            if (j == 0 && no[c] >= 1 && !(ok = wait(bar(B_OE + c), (no[c] - 1) & 1))) break;
+            fence_after();
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              mma_ts(tmem + Lay::O + Lay::O_STEP * c, tmem + Lay::P + Lay::P_STEP * c + 8 * kk,
+                     sdesc(sV + kk * 2048, kBox, 1024), ID_PV, (j | kk) != 0);
+            mma_commit(bar(B_OD + c));
+            mma_commit(bar(B_VE + sv));
+            ++np[c];
+            if (j + 1 < ch.n[c]) {
+              ok = issue_s(c, n + 1, false, j + 2 == ch.n[c]);
+            } else {
+              ++no[c];
+              if (j + 1 < ch.nt) mma_commit(bar(B_KE + (n + 1) % NS_K));
+              if (nx.n[c] > 0) {
+                ok = issue_s(c, kb + ch.nt, true, nx.n[c] == 1);
+                ahead[c] = i + 1;
+              }
+            }
+          }
+        }
+        kb += ch.nt;
+      }
+      mma_commit(bar(B_DRAIN));
+      mbar_drain(bar(B_DRAIN), 0);
+    } else if (warp >= 10) {
+      // ============================== V of cut tiles ==============================
+      const int half = warp - 10, chunks = p.dv >> 3;
+      int kb = 0, cut = 0;
+      bool ok = true;
+      for (int i = w0; ok && i < w1; ++i) {
+        const PfPiece w = p.pieces[i];
+        const PfChains ch = chains_of(w, p.ppt);
+        for (int j = 0; ok && j < ch.nt; ++j) {
+          const int t = w.t0 + j;
+          if (!tile_cut(w, t)) continue;
+          const int sv = (kb + j) % NS_V;
+          if (!(ok = wait_all(bar(B_VC + (cut & 3)), (cut >> 2) & 1))) break;
+          unsigned char* sV = smem + Lay::OFF_V + sv * Lay::V_BYTES;
+          const int r0 = max(0, w.vis0 - t * kKeys);         // rows below: every row of the item sees them
+          const int r1 = min(kKeys, ch.vis_max - t * kKeys);  // rows from here on: none does
+          uint32_t bad = 0;
+          for (int e = half * 32 + lane; e < (kKeys - r0) * chunks; e += 64) {
+            const int r = r0 + e / chunks, k = e % chunks;
+            uint4* at = reinterpret_cast<uint4*>(sV + (k >> 3) * kBox + r * 128 + (((k & 7) ^ (r & 7)) << 4));
+            if (r >= r1) {
+              *at = make_uint4(0, 0, 0, 0);
+              continue;
+            }
+            uint4 x = *at;
+            uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
+            uint32_t any = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t f = nonfinite_bf16x2(xw[q]);
+              any |= f;
+              if (f & 0x8000u) xw[q] &= 0xFFFF0000u;
+              if (f & 0x80000000u) xw[q] &= 0x0000FFFFu;
+            }
+            if (any) *at = x;
+            bad |= any;
+          }
+          if (bad) s_bad[i & 3] = i + 1;
+          fence_proxy_async();  // these reads and writes before the tensor core's reads and the slot's next copy
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_VF + sv));
+          ++cut;
+        }
+        kb += ch.nt;
+      }
+    }
+    __syncwarp();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    // ============================== softmax ==============================
+    const int c = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = tlane + Lay::S + 128 * c, tP = tlane + Lay::P + Lay::P_STEP * c, tO = tlane + Lay::O + Lay::O_STEP * c;
+    const int pos = row / p.rep, head = row - pos * p.rep;
+    int n_s = 0;  // tiles of this chain so far
+    bool ok = true;
+    int i = w0;
+    for (; i < w1; ++i) {
+      const PfPiece w = p.pieces[i];
+      const PfChains ch = chains_of(w, p.ppt);
+      if (!ch.active[c]) continue;
+      const int lpos = c * p.ppt + pos;                       // position within the item
+      const bool have = pos < p.ppt && lpos < w.npos;
+      const int vis = have ? w.vis0 + lpos : 0;               // keys that this row sees
+      float m_true = -INFINITY, m_ref = -INFINITY;
+      float l = 0.f;
+      const int nt = ch.n[c];
+      for (int j = 0; j < nt; ++j, ++n_s) {
+        if (!(ok = wait_all_inline(bar(B_SF + c), n_s & 1))) break;
+        fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld32p(tS + 32 * x, s + 32 * x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) touch16(s + 16 * x);
+        if (!ALIAS) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_SR + c));
+        }
+        const int kb = (w.t0 + j) * kKeys;
+        if (kb + kKeys > ch.vis_first[c]) {
+          const int nvis = vis - kb;  // keys of the tile that this row sees
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x >= nvis) s[x] = 0xFF800000u;  // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) mx[a] = a == 0 ? m_true : __uint_as_float(s[a]);
+        mx[0] = max3_nan(mx[0], __uint_as_float(s[0]), __uint_as_float(s[4]));
+#pragma unroll
+        for (int a = 1; a < 4; ++a) mx[a] = max3_nan(mx[a], __uint_as_float(s[4 + a]), __uint_as_float(s[4 + a]));
+#pragma unroll
+        for (int x = 8; x < 128; x += 8)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) mx[a] = max3_nan(mx[a], __uint_as_float(s[x + a]), __uint_as_float(s[x + 4 + a]));
+        m_true = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        // the reference moves when it has to: at once from "none", and when outgrown by 2^8 or more
+        const bool grow = (m_true - m_ref) * p.sl2 > kRescale;  // -inf - -inf is NaN: false
+        if (j == 0) {
+          if (grow) m_ref = m_true;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? m_true : m_ref;
+          const float alpha = m_ref == -INFINITY ? 0.f : (grow ? fast_exp2((m_ref - m_new) * p.sl2) : 1.f);
+          if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
+          fence_after();
+          for (int x = 0; x < p.dv; x += 16) {
+            uint32_t o[16];
+            tmem_ld16(tO + x, o);
+            tmem_wait_ld();
+            touch16(o);
+#pragma unroll
+            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+            tmem_st16(tO + x, o);
+          }
+          tmem_wait_st();
+          l *= alpha;
+          m_ref = m_new;
+        }
+        const float mb = m_ref == -INFINITY ? 0.f : -m_ref * p.sl2;
+        const uint64_t sl2 = pack2(p.sl2, p.sl2), mb2 = pack2(mb, mb);
+        uint64_t l2[2] = {pack2(l, 0.f), pack2(0.f, 0.f)};
+        // PV of the tile before has read P (and every phase of the barrier is seen, so that its parity says which)
+        if (j > 0 && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) {
+            const uint64_t y =
+                fma2(pack2(__uint_as_float(s[64 * h + 2 * x]), __uint_as_float(s[64 * h + 2 * x + 1])), sl2, mb2);
+            float a, b;
+            unpack2(y, a, b);
+            a = fast_exp2(a);
+            b = fast_exp2(b);
+            l2[x & 1] = add2(l2[x & 1], pack2(a, b));
+            pk[x] = pack_bf16(a, b);
+          }
+          tmem_st32p(tP + 32 * h, pk);
+        }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PF + c));
+        l2[0] = add2(l2[0], l2[1]);
+        float la, lb;
+        unpack2(l2[0], la, lb);
+        l = la + lb;
+      }
+      if (!ok) break;
+      // ---- epilogue ----
+      if (nt > 0) {
+        if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
+        fence_after();
+      }
+      // a NaN or +infinity among the row's scores makes the row NaN
+      const bool lost = isnan(m_true) || m_true == INFINITY;
+      const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
+      const size_t tok = (size_t)w.q0 + lpos;
+      const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : (vis <= 0 ? 0.f : 1.f / l));
+      float* po = p.ws_o + ((size_t)w.slot * 2 * kRows + c * kRows + row) * p.dv;  // used with a slot only
+      __nv_bfloat16* go = p.out + (tok * p.n_q + w.kvh * p.rep + head) * p.dv;
+      for (int x = 0; x < p.dv; x += 16) {
+        uint32_t o[16];
+        if (nt > 0) {
+          tmem_ld16(tO + x, o);
+          tmem_wait_ld();
+          touch16(o);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 16; ++y) o[y] = 0;
+        }
+        if (!have) continue;
+        if (bad) {  // non-finite values of the partly visible V rows, to the rows that see them
+          const int k_lo = max(w.vis0, w.t0 * kKeys), k_hi = min(vis, w.t1 * kKeys);
+          for (int k = max(k_lo, 0); k < k_hi; ++k) {
+            const __nv_bfloat16* vr = p.v + (int64_t)(w.k0 + k) * p.v_tok + w.kvh * p.v_head + x;
+            for (int y = 0; y < 16; ++y) {
+              const float f = __bfloat162float(vr[y]);
+              if (!(fabsf(f) < INFINITY)) {
+#pragma unroll
+                for (int z = 0; z < 16; ++z)
+                  if (z == y) o[z] = __float_as_uint(__uint_as_float(o[z]) + f);
+              }
+            }
+          }
+        }
+        if (w.slot >= 0) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            reinterpret_cast<uint4*>(po + x)[y] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+        } else {
+          uint32_t h[8];
+#pragma unroll
+          for (int y = 0; y < 8; ++y)
+            h[y] = vis <= 0 ? 0u : pack_bf16(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
+          reinterpret_cast<uint4*>(go + x)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+          reinterpret_cast<uint4*>(go + x)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      }
+      if (w.slot >= 0 && have) {
+        float* ml = p.ws_ml + ((size_t)w.slot * 2 * kRows + c * kRows + row) * 2;
+        ml[0] = lost ? NAN : (m_ref == -INFINITY ? -INFINITY : m_ref * p.sl2);
+        ml[1] = l;
+      }
+      if (nt > 0) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_OE + c));
+      }
+    }
+    if (!ok) {  // the rows that this chain still owed become NaN
+      for (; i < w1; ++i) {
+        const PfPiece w = p.pieces[i];
+        const int lpos = c * p.ppt + pos;
+        if (pos >= p.ppt || lpos >= w.npos) continue;
+        if (w.slot >= 0) {
+          p.ws_ml[((size_t)w.slot * 2 * kRows + c * kRows + row) * 2] = NAN;
+          continue;
+        }
+        __nv_bfloat16* go = p.out + (((size_t)w.q0 + lpos) * p.n_q + w.kvh * p.rep + head) * p.dv;
+        for (int x = 0; x < p.dv; ++x) go[x] = __float2bfloat16(NAN);
+      }
+    }
+  }
+  // every role reaches this point warp-converged
+  fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Joins the records of the items that were cut along the keys: one warp per row, with w_s = 2^(m_s - max m),
+// o = sum_s w_s O_s / sum_s w_s l_s. Bound by reading the records (fp32).
+__global__ void __launch_bounds__(256) palu_prefill_merge_kernel(const PfMerge* merges, const PfParams p) {
+  const PfMerge w = merges[blockIdx.x];
+  const int lane = threadIdx.x & 31;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < 2 * kRows; r += gridDim.y * 8) {
+    const int c = r >> 7, row = r & 127, pos = row / p.rep, head = row - pos * p.rep, lpos = c * p.ppt + pos;
+    if (pos >= p.ppt || lpos >= w.npos) continue;
+    const bool empty = w.vis0 + lpos <= 0;
+    float m = -INFINITY;
+    bool lost = false;
+    for (int s = 0; s < w.n; ++s) {
+      const float ms = p.ws_ml[((size_t)(w.slot0 + s) * 2 * kRows + r) * 2];
+      lost |= isnan(ms);
+      m = fmaxf(m, ms);
+    }
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    const int x = lane * 4;
+    for (int s = 0; s < w.n; ++s) {
+      const size_t rec = (size_t)(w.slot0 + s) * 2 * kRows + r;
+      const float ms = p.ws_ml[rec * 2];
+      if (ms == -INFINITY) continue;  // the row saw nothing of this piece
+      const float wt = fast_exp2(ms - m);
+      l += wt * p.ws_ml[rec * 2 + 1];
+      if (x < p.dv) {
+        const float4 v = *reinterpret_cast<const float4*>(p.ws_o + rec * p.dv + x);
+        o[0] += wt * v.x;
+        o[1] += wt * v.y;
+        o[2] += wt * v.z;
+        o[3] += wt * v.w;
+      }
+    }
+    if (x < p.dv) {
+      const float inv = lost ? NAN : 1.f / l;
+      uint2 h = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+      if (empty) h = make_uint2(0u, 0u);
+      *reinterpret_cast<uint2*>(p.out + (((size_t)w.q0 + lpos) * p.n_q + w.kvh * p.rep + head) * p.dv + x) = h;
+    }
+  }
+}
+
+}  // namespace pf
+}  // namespace palu

@@ -25,6 +25,7 @@ EXPORTED = ("palu_decode_attn", "palu_decode_attn_static", "palu_decode_attn_pag
             "palu_read_status",
             "palu_set_wait_limit", "palu_decode_attn_f8", "palu_quantize_latents_f8", "palu_append_latents_f8",
             "palu_decode_attn_f4", "palu_quantize_latents_f4", "palu_append_latents_f4",
+            "palu_plan_prefill", "palu_prefill_workspace_bytes", "palu_prefill_attn",
             "palu_last_error", "palu_version")
 PALU_KERNEL_AUTO, PALU_KERNEL_MMA, PALU_KERNEL_TC = 0, 1, 2
 PALU_ROPE_ABSOLUTE, PALU_ROPE_CHUNK_RELATIVE = 0, 1
@@ -39,6 +40,13 @@ class DecodeDims(ctypes.Structure):
 class PageTable(ctypes.Structure):
     _fields_ = [("table", ctypes.c_void_p), ("table_ld", ctypes.c_int32), ("block_size", ctypes.c_int32),
                 ("n_blocks", ctypes.c_int32)]
+
+
+class PrefillPlanInfo(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int64) for n in ("bytes", "q_tokens", "k_tokens", "off_start", "off_pieces", "off_merges",
+                                               "off_tiles")]
+                + [(n, ctypes.c_int32) for n in ("n_seq", "n_q_heads", "n_kv_heads", "pos_per_chain", "n_ctas", "n_pieces",
+                                                 "n_merges", "n_slots", "n_tiles")])
 
 
 _lib = None
@@ -102,6 +110,14 @@ def load() -> ctypes.CDLL:
     lib.palu_kernel_for.restype = i32
     lib.palu_read_status.argtypes = [vp, ctypes.POINTER(i32), vp]
     lib.palu_read_status.restype = ctypes.c_int
+    plan_p = ctypes.POINTER(PrefillPlanInfo)
+    i32_p = ctypes.POINTER(i32)
+    lib.palu_plan_prefill.argtypes = [i32_p, i32_p, i32_p, i32, i32, i32, i32, vp, sz, plan_p]
+    lib.palu_plan_prefill.restype = ctypes.c_int
+    lib.palu_prefill_workspace_bytes.argtypes = [plan_p, i32]
+    lib.palu_prefill_workspace_bytes.restype = sz
+    lib.palu_prefill_attn.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, plan_p, vp, vp, sz, f32, vp]
+    lib.palu_prefill_attn.restype = ctypes.c_int
     lib.palu_last_error.argtypes = []
     lib.palu_last_error.restype = ctypes.c_char_p
     lib.palu_version.argtypes = []

@@ -9,7 +9,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / "csrc"
 OUT = PKG / "libpalu_b200.so"
-SOURCES = ["palu_abi.cu"]
+SOURCES = ["palu_abi.cu", "palu_serve.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -21,7 +21,7 @@ def nvcc() -> str:
 
 def command(verbose_ptxas: bool = False) -> list:
     cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "--expt-relaxed-constexpr", "-o", str(OUT)] + [str(CSRC / s) for s in SOURCES]
+           "--expt-relaxed-constexpr", "--threads", "0", "-o", str(OUT)] + [str(CSRC / s) for s in SOURCES]
     if verbose_ptxas:
         cmd.insert(1, "-Xptxas=-v")
     return cmd
@@ -31,7 +31,7 @@ def stale() -> bool:
     if not OUT.exists():
         return True
     t = OUT.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list((PKG.parent.parent / "include").glob("*.h"))
+    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((PKG.parent.parent / "include").glob("*.h"))
     return any(p.stat().st_mtime > t for p in deps)
 
 

@@ -1,0 +1,141 @@
+"""Prefill of packed prompts: the batch's plan and the causal attention over it.
+
+A packed batch holds sequences of different lengths one after another, without padding: sequence s has ``q_lens[s]``
+query positions and ``k_lens[s]`` keys, its last query aligned with its last key (a prompt: equal lengths; a prompt
+chunk behind a cached prefix: more keys than queries). ``PrefillPlan`` lays the batch's work out once, on the host;
+every layer of a forward pass then uses it (``prefill_attn``). The reference prefills one user's padded prompt at a
+time with the stock attention op (palu_tt/attention.py:382-516).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence
+
+import torch
+
+from palu_b200 import _lib
+
+HEAD_DIM = 128
+
+
+def _lengths(x, what: str):
+    """Host lengths (a sequence or an integer CPU tensor) as a ctypes int32 array."""
+    if isinstance(x, torch.Tensor):
+        if x.is_cuda:
+            raise RuntimeError(f"{what} must be on the host (a sequence or a CPU tensor): the plan is laid out there")
+        x = x.reshape(-1).tolist()
+    x = [int(v) for v in x]
+    if any(not -2**31 <= v < 2**31 for v in x):
+        raise RuntimeError(f"{what} must fit 32 bits")
+    return (ctypes.c_int32 * len(x))(*x), x
+
+
+class PrefillPlan:
+    """The work of one packed batch, laid out for the GPU (palu_plan_prefill).
+
+    ``q_lens`` / ``k_lens``: host lengths per sequence (``k_lens`` None: equal to ``q_lens``). ``rows``: the cache row of
+    each sequence, for ``rebuild_kv`` (None: 0, 1, ...). Building a plan copies it to ``device`` and waits for the copy, so
+    build it outside a CUDA graph capture; it can then be used on any stream of that device, by any number of calls, also
+    at the same time."""
+
+    def __init__(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, n_q_heads: int, n_kv_heads: int,
+                 rows: Optional[Sequence[int]] = None, device="cuda"):
+        ql, self.q_lens = _lengths(q_lens, "q_lens")
+        kl, self.k_lens = (ql, self.q_lens) if k_lens is None else _lengths(k_lens, "k_lens")
+        if len(self.q_lens) != len(self.k_lens):
+            raise RuntimeError(f"q_lens and k_lens must have the same length, got {len(self.q_lens)} and {len(self.k_lens)}")
+        rl, self.rows = (None, list(range(len(self.q_lens)))) if rows is None else _lengths(rows, "rows")
+        if len(self.rows) != len(self.q_lens):
+            raise RuntimeError(f"rows must name one cache row per sequence, got {len(self.rows)} for {len(self.q_lens)}")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise RuntimeError(f"palu_b200 runs on CUDA tensors only (no CPU path); got a plan for {self.device}")
+        self.info = _lib.PrefillPlanInfo()
+        lib, n = _lib.load(), len(self.q_lens)
+        if torch.cuda.is_available():
+            if self.device.index is None:
+                self.device = torch.device("cuda", torch.cuda.current_device())
+            ctas = torch.cuda.get_device_properties(self.device).multi_processor_count
+        else:
+            ctas = 0
+        size = 1 << 16
+        while True:
+            host = torch.empty(size, dtype=torch.uint8)
+            st = lib.palu_plan_prefill(ql, kl, rl, n, int(n_q_heads), int(n_kv_heads), ctas, host.data_ptr(), size,
+                                       ctypes.byref(self.info))
+            if st != _lib.PALU_ERR_WORKSPACE:
+                break
+            size = int(self.info.bytes)
+        _lib.check(st)
+        self.q_tokens, self.k_tokens = int(self.info.q_tokens), int(self.info.k_tokens)
+        self.n_q_heads, self.n_kv_heads = int(n_q_heads), int(n_kv_heads)
+        self._ws_bytes = {}
+        self.host = host[:int(self.info.bytes)]
+        self.data = self.host.to(self.device)
+        stream = torch.cuda.current_stream(self.device)
+        stream.synchronize()
+        self._stream = stream.cuda_stream
+        self.info_ptr = ctypes.byref(self.info)
+
+    def workspace_bytes(self, d_v: int) -> int:
+        n = self._ws_bytes.get(d_v)
+        if n is None:
+            n = self._ws_bytes[d_v] = int(_lib.load().palu_prefill_workspace_bytes(self.info_ptr, d_v))
+        return n
+
+    def use_on(self, stream: int) -> None:
+        """Keep the plan's memory until work queued on ``stream`` is done, if that is not the stream it was made on."""
+        if stream != self._stream and not torch.cuda.is_current_stream_capturing():
+            self.data.record_stream(torch.cuda.current_stream(self.device))
+
+    def status(self) -> int:
+        """Read and clear the plan's status word: nonzero when a bounded device wait of a call expired (the rows that it
+        kept from being computed are NaN)."""
+        return _lib.read_status(self.data)
+
+
+def _heads(t: torch.Tensor, what: str, tokens: int, heads: int, width: Optional[int], device) -> torch.Tensor:
+    """A bf16 [tokens, heads, width] tensor on the plan's device, its last dimension contiguous and its rows 16-byte
+    aligned (copied where they are not)."""
+    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or (width is not None and t.shape[2] != width):
+        raise RuntimeError(f"{what} must be [{tokens}, {heads}, {width if width is not None else 'd_v'}], got {tuple(t.shape)}")
+    if t.device != device:
+        raise RuntimeError(f"{what} is on {t.device}, the plan on {device}")
+    if t.dtype != torch.bfloat16:
+        raise RuntimeError(f"{what} must be bf16, got {t.dtype}")
+    s = t.stride()
+    if s[2] != 1 or s[1] % 8 or s[0] % 8 or s[0] <= 0 or s[1] <= 0 or t.data_ptr() % 16:
+        t = t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone()
+    return t
+
+
+def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PrefillPlan, *, scale: Optional[float] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of a packed batch (palu_prefill_attn): q [q_tokens, n_q, 128], k [k_tokens, n_kv, 128] (both already
+    rotated), v [k_tokens, n_kv, d_v] bf16, d_v a multiple of 16 up to 128 -> [q_tokens, n_q, d_v] bf16.
+
+    Query i of a sequence sees its keys 0 .. i + k_len - q_len; one that sees none gives 0. What lies behind a query's
+    last key does not reach its result, whatever it holds. q, k and v may be strided (slices of a fused projection);
+    the products accumulate in fp32, the probabilities are rounded to bf16 for the second one."""
+    _lib.require_cuda(q, k, v, out)
+    q = _heads(q, "q", plan.q_tokens, plan.n_q_heads, HEAD_DIM, plan.device)
+    k = _heads(k, "k", plan.k_tokens, plan.n_kv_heads, HEAD_DIM, plan.device)
+    v = _heads(v, "v", plan.k_tokens, plan.n_kv_heads, None, plan.device)
+    d_v = v.shape[2]
+    shape = (plan.q_tokens, plan.n_q_heads, d_v)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    elif tuple(out.shape) != shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
+        raise RuntimeError(f"out must be a contiguous bf16 {shape} tensor on {q.device}")
+    if q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return prefill_attn(q, k, v, plan, scale=scale, out=out)
+    need = plan.workspace_bytes(d_v)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    stream = _lib.stream_handle(q.device)
+    plan.use_on(stream)
+    _lib.check(_lib.load().palu_prefill_attn(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+        v.stride(1), out.data_ptr(), d_v, plan.info_ptr, plan.data.data_ptr(), _lib.ptr(ws), need,
+        HEAD_DIM ** -0.5 if scale is None else float(scale), stream))
+    return out
