@@ -294,7 +294,7 @@ typedef struct palu_prefill_plan {
   int64_t bytes, q_tokens, k_tokens;
   int64_t off_start, off_pieces, off_merges, off_tiles; /* of the buffer's parts */
   int32_t n_seq, n_q_heads, n_kv_heads, pos_per_chain;
-  int32_t n_ctas, n_pieces, n_merges, n_slots, n_tiles;
+  int32_t n_ctas, n_pieces, n_merges, n_slots, n_tiles, max_k_len, max_row;
 } palu_prefill_plan;
 int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_t* rows, int32_t n_seq, int32_t n_q_heads,
                       int32_t n_kv_heads, int32_t n_ctas, void* buf, size_t buf_bytes, palu_prefill_plan* plan);
@@ -311,6 +311,71 @@ size_t palu_prefill_workspace_bytes(const palu_prefill_plan* plan, int32_t d_v);
 int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                       const void* v, int64_t v_tok, int64_t v_head, void* out, int32_t d_v, const palu_prefill_plan* plan,
                       void* plan_data, void* workspace, size_t workspace_bytes, float scale, palu_stream_t stream);
+
+/*
+ * Packed keys and values of cached latents, for palu_prefill_attn behind a cached prefix: for the k_lens[s] positions of
+ * each sequence s of the plan, read from cache row rows[s],
+ *   K[t][h] = R_pos (k_lat[g][pos] U_k[h]),   V[t][h] = v_lat[g][pos] U_v[h],   g = h / (n_kv_heads / n_groups).
+ * k_lat, v_lat: bf16 caches as palu_decode_attn's ([B][n_groups][max_seq][r]; every k_lens[s] at most max_seq and every
+ * rows[s] below B) or, with `pages`, palu_decode_attn_paged's (table rows of at least ceil(max_seq / block_size) entries;
+ * an entry outside [0, n_blocks) reads as zero latents). u_k [n_kv_heads][r_k][128] and u_v [n_kv_heads][r_v][128] or
+ * NULL, bf16; cos, sin [>= longest k_len][128] f32, each frequency at columns 2j and 2j + 1. k_out
+ * [k_tokens][n_kv_heads][128]; v_out [k_tokens][n_kv_heads][128], or [k_tokens][n_groups][r_v] without u_v (the latents
+ * themselves, absorbed V). r_k, r_v multiples of 16 up to 256. fp32 accumulation and rotation, one rounding to bf16.
+ */
+int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const void* u_v, const float* cos, const float* sin,
+                    const palu_page_table* pages, const palu_prefill_plan* plan, const void* plan_data, void* k_out, void* v_out,
+                    int32_t n_groups, int32_t r_k, int32_t r_v, int32_t max_seq, palu_stream_t stream);
+
+/*
+ * Log probability of one given token per row of logits, the entropy of the row's distribution (nats) and its `top`
+ * highest log probabilities with their token ids, highest first, equal logits by the lower id (reference: none; its
+ * generation is greedy, palu_tt/generate.py:53-62).
+ *   logits [rows] rows of `ld` elements, the first `vocab` used, PALU_BF16 or PALU_F32, any alignment of its type
+ *   tokens [rows] int64 (tokens64 nonzero) or int32; negative: no token, log probability 0; >= vocab: NaN
+ *   logprob, entropy [rows]; top_logprob [rows][top], top_id [rows][top] (may be NULL when top is 0; top <= 32)
+ * A logit of -inf has probability 0. A row whose logits are all -inf, or that holds a NaN or +inf, has no distribution:
+ * its log probabilities and entropy are NaN (its ids still order the logits, NaN highest).
+ */
+int palu_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t rows, int32_t vocab, const void* tokens, int32_t tokens64,
+                        int32_t top, float* logprob, float* entropy, float* top_logprob, int64_t* top_id, palu_stream_t stream);
+
+/*
+ * Pages of paged caches. A pool is device memory of the caller:
+ *   table   [rows][blocks_per_row] int32, the page table of palu_decode_attn_paged; -1: no page (initially everywhere)
+ *   refs    [n_blocks] int32: how many table entries name a page (initially 0)
+ *   mapped  [rows] int32: a row's mapped entries, which come first (initially 0)
+ *   status  [1] int32 (initially 0): bit 0 set when pages ran out (the row keeps what it got; a fork is left out), bit 1
+ *           when a fork's parent held fewer positions than asked for, bit 2 when a child was not empty (both left out)
+ * A page taken is always the lowest free one, in the order of the call's rows. Row lists are host memory, read before
+ * the call returns. Calls on one pool, and the work that reads its caches, have to be ordered by the caller (one stream).
+ *
+ * palu_reserve_pages: rows[i] gets pages up to lens[i] positions. palu_fork_pages: children[i], which is empty, shares
+ * parents[i]'s pages of the first lens[i] positions (read-only from then on, for both); a page they fill only partly is
+ * copied into a page of the child's own, in every cache. A row may be the parent of several children, not parent and
+ * child at once. palu_free_pages: the rows give up their pages; those that nothing names any more are free.
+ * palu_compact_pages: pages in use move to the lowest places, in every cache, and the table and counts follow.
+ * workspace: palu_page_workspace_bytes(n_blocks) bytes, 16-byte aligned, the pool's own.
+ * palu_copy_pages: block src[i] to block dst[i] in every cache (no pool); no block is copied to twice, or copied both from
+ * and to. A cache: n_blocks blocks of block_bytes bytes, block_stride bytes apart, any type.
+ */
+typedef struct palu_page_pool {
+  int32_t *table, *refs, *mapped, *status;
+  int32_t rows, blocks_per_row, n_blocks, block_size;
+} palu_page_pool;
+typedef struct palu_page_cache {
+  void* base;
+  int64_t block_stride, block_bytes;
+} palu_page_cache;
+size_t palu_page_workspace_bytes(int32_t n_blocks);
+int palu_reserve_pages(const palu_page_pool* pool, const int32_t* rows, const int32_t* lens, int32_t n, palu_stream_t stream);
+int palu_fork_pages(const palu_page_pool* pool, const palu_page_cache* caches, int32_t n_caches, const int32_t* parents,
+                    const int32_t* children, const int32_t* lens, int32_t n, void* workspace, size_t workspace_bytes, palu_stream_t stream);
+int palu_free_pages(const palu_page_pool* pool, const int32_t* rows, int32_t n, palu_stream_t stream);
+int palu_compact_pages(const palu_page_pool* pool, const palu_page_cache* caches, int32_t n_caches, void* workspace,
+                       size_t workspace_bytes, palu_stream_t stream);
+int palu_copy_pages(const palu_page_cache* caches, int32_t n_caches, int32_t n_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    palu_stream_t stream);
 
 /*
  * Select the decode kernel family for subsequent calls in this process (PALU_KERNEL_AUTO by default:

@@ -6,7 +6,10 @@
 
 #include "../../include/palu_b200.h"
 #include "abi_common.h"
+#include "logprobs.cuh"
+#include "pages.cuh"
 #include "prefill_tc.cuh"
+#include "rebuild.cuh"
 
 using namespace palu::abi;
 
@@ -142,6 +145,102 @@ void make_lists(const int32_t* q_lens, const int32_t* k_lens, const int32_t* row
   }
 }
 
+// ---- pages --------------------------------------------------------------------------------------------
+
+int check_pool(const palu_page_pool* q, palu::pg::Pool& p) {
+  if (!q) return fail(PALU_ERR_INVALID, "pool is NULL");
+  if (!q->table || !q->refs || !q->mapped || !q->status) return fail(PALU_ERR_INVALID, "pool: table, refs, mapped and status must be set");
+  if (q->rows <= 0 || q->blocks_per_row <= 0 || q->n_blocks <= 0 || q->block_size <= 0)
+    return fail(PALU_ERR_INVALID, "pool: rows, blocks_per_row, n_blocks and block_size must be positive (got %d, %d, %d, %d)", q->rows,
+                q->blocks_per_row, q->n_blocks, q->block_size);
+  p = {q->table, q->refs, q->mapped, q->status, q->rows, q->blocks_per_row, q->n_blocks, q->block_size};
+  return PALU_OK;
+}
+
+int check_rows(const char* what, const int32_t* rows, const int32_t* lens, int n, const palu::pg::Pool& p) {
+  if (n < 0 || (n > 0 && !rows)) return fail(PALU_ERR_INVALID, "%s must hold n entries", what);
+  for (int i = 0; i < n; ++i) {
+    if (rows[i] < 0 || rows[i] >= p.rows) return fail(PALU_ERR_INVALID, "%s: row %d is outside [0, %d)", what, rows[i], p.rows);
+    if (lens && (lens[i] < 0 || lens[i] > (int64_t)p.per_row * p.page_size))
+      return fail(PALU_ERR_INVALID, "%s: a row of %d blocks of %d cannot hold %d positions", what, p.per_row, p.page_size, lens[i]);
+  }
+  std::vector<int32_t> s(rows, rows + n);
+  std::sort(s.begin(), s.end());
+  for (int i = 1; i < n; ++i)
+    if (s[i] == s[i - 1]) return fail(PALU_ERR_INVALID, "%s: row %d is named twice", what, s[i]);
+  return PALU_OK;
+}
+
+// Caches of one launch, and whether all of them take 16-byte accesses.
+int check_caches(const palu_page_cache* caches, int n, int n_blocks) {
+  if (n < 0 || (n > 0 && !caches)) return fail(PALU_ERR_INVALID, "caches must hold n_caches entries");
+  for (int i = 0; i < n; ++i)
+    if (!caches[i].base || caches[i].block_bytes <= 0 || (n_blocks > 1 && caches[i].block_stride < caches[i].block_bytes))
+      return fail(PALU_ERR_INVALID, "cache %d: blocks of %lld bytes every %lld bytes", i, (long long)caches[i].block_bytes,
+                  (long long)caches[i].block_stride);
+  return PALU_OK;
+}
+bool fill_caches(const palu_page_cache* caches, int n, palu::pg::Caches& a, int64_t& most) {
+  a.n = n;
+  most = 0;
+  bool wide = true;
+  for (int i = 0; i < n; ++i) {
+    a.c[i] = {static_cast<unsigned char*>(caches[i].base), caches[i].block_stride, caches[i].block_bytes};
+    most = std::max(most, caches[i].block_bytes);
+    wide &= (reinterpret_cast<uintptr_t>(caches[i].base) | caches[i].block_stride | caches[i].block_bytes) % 16 == 0;
+  }
+  return wide;
+}
+// Thread blocks per cache: enough for 8 of 256 threads on every SM over all caches, no more than there are units.
+int copy_grid(int n_caches, int64_t moves, int64_t most) {
+  const int64_t units = moves * ((most + palu::pg::kPart - 1) / palu::pg::kPart);
+  const int64_t fill = (8LL * device_sms() + n_caches - 1) / std::max(1, n_caches);
+  return (int)std::max<int64_t>(1, std::min(units, fill));
+}
+
+template <class K, class... A>
+int launch_dependent(const char* what, K kern, dim3 grid, int threads, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return cuda_check(what);
+  return cuda_check(what);
+}
+
+// The move list behind a state change, applied to every cache (and the table, with a target array).
+int apply_moves(const palu::pg::Pool& p, const palu::pg::Moves& mv, const int32_t* target, const palu_page_cache* caches, int n_caches,
+                int64_t most_moves, cudaStream_t stream) {
+  for (int i = 0; i < n_caches || (i == 0 && target); i += palu::pg::kMaxCaches) {
+    palu::pg::Caches a;
+    int64_t most;
+    const int n = std::min(palu::pg::kMaxCaches, n_caches - i);
+    const bool wide = fill_caches(caches + i, n, a, most);
+    const dim3 grid(copy_grid(n, most_moves, std::max<int64_t>(most, 1)), std::max(1, n));
+    const int32_t* t = i == 0 ? target : nullptr;
+    const int st = wide ? launch_dependent("page move launch", palu::pg::palu_move_pages_kernel<uint4>, grid, palu::pg::kCopyThreads, stream, p, mv, t, a)
+                        : launch_dependent("page move launch", palu::pg::palu_move_pages_kernel<uint8_t>, grid, palu::pg::kCopyThreads, stream, p, mv, t, a);
+    if (st) return st;
+  }
+  return PALU_OK;
+}
+
+// Runs f and turns a C++ exception (out of host memory) into a status.
+template <class F>
+int guarded(F f) {
+  g_err.clear();
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return fail(PALU_ERR_INVALID, "out of host memory");
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -157,12 +256,15 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
   if (rep > palu::pf::kRows) return fail(PALU_ERR_INVALID, "at most 128 query heads per KV head are supported, got %d", rep);
   if (n_ctas < 0 || n_ctas > 4096) return fail(PALU_ERR_INVALID, "n_ctas must be in [0, 4096], got %d", n_ctas);
   int64_t tq = 0, tk = 0;
+  int32_t longest = 0, last_row = -1;
   for (int s = 0; s < n_seq; ++s) {
     if (q_lens[s] < 0 || k_lens[s] < 0)
       return fail(PALU_ERR_INVALID, "sequence %d: lengths must not be negative (got %d queries, %d keys)", s, q_lens[s], k_lens[s]);
     if (rows && rows[s] < 0) return fail(PALU_ERR_INVALID, "sequence %d: cache row %d is negative", s, rows[s]);
     tq += q_lens[s];
     tk += k_lens[s];
+    longest = std::max(longest, k_lens[s]);
+    last_row = std::max(last_row, rows ? rows[s] : s);
   }
   if (tq > (1 << 28) || tk > (1 << 28)) return fail(PALU_ERR_INVALID, "at most 2^28 packed tokens are supported");
   try {
@@ -172,6 +274,8 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
     plan->q_tokens = tq;
     plan->k_tokens = tk;
     plan->n_seq = n_seq;
+    plan->max_k_len = longest;
+    plan->max_row = last_row;
     plan->n_q_heads = n_q_heads;
     plan->n_kv_heads = n_kv_heads;
     plan->pos_per_chain = ppt;
@@ -276,6 +380,222 @@ int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* 
     return cuda_check("prefill merge launch");
   }
   return PALU_OK;
+}
+
+int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const void* u_v, const float* cos, const float* sin,
+                    const palu_page_table* pages, const palu_prefill_plan* plan, const void* plan_data, void* k_out, void* v_out,
+                    int32_t n_groups, int32_t r_k, int32_t r_v, int32_t max_seq, palu_stream_t stream) {
+  g_err.clear();
+  if (!plan || !plan_data) return fail(PALU_ERR_INVALID, "rebuild: plan and its device data must be set");
+  if (n_groups <= 0 || plan->n_kv_heads % n_groups != 0)
+    return fail(PALU_ERR_INVALID, "heads_per_group: %d latent heads do not divide %d KV heads", n_groups, plan->n_kv_heads);
+  if (r_k < 16 || r_k > 256 || r_k % 16 != 0) return fail(PALU_ERR_INVALID, "r_k must be a multiple of 16 in [16, 256], got %d", r_k);
+  if (r_v < 16 || r_v > 256 || r_v % 16 != 0) return fail(PALU_ERR_INVALID, "r_v must be a multiple of 16 in [16, 256], got %d", r_v);
+  if (n_groups != plan->n_kv_heads && !u_v)
+    return fail(PALU_ERR_INVALID, "grouped latents (%d groups for %d KV heads) need u_v", n_groups, plan->n_kv_heads);
+  if (max_seq <= 0 || plan->max_k_len > max_seq)
+    return fail(PALU_ERR_INVALID, "rebuild: max_seq %d must be positive and hold the longest sequence's %d keys", max_seq, plan->max_k_len);
+  if (plan->n_tiles == 0) return PALU_OK;
+  if (!k_lat || !v_lat || !u_k || !cos || !sin || !k_out || !v_out) return fail(PALU_ERR_INVALID, "rebuild: every pointer must be set");
+  for (const void* x : {k_lat, v_lat, u_k, u_v, plan_data, (const void*)k_out, (const void*)v_out})
+    if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return fail(PALU_ERR_INVALID, "rebuild: pointers must be 16-byte aligned");
+  palu::rb::Params p;
+  p.page_table = nullptr;
+  p.table_ld = p.blk_shift = p.n_blocks = 0;
+  if (pages) {
+    const int bs = pages->block_size;
+    if (!pages->table || pages->n_blocks <= 0 || (bs != 16 && bs != 32 && bs != 64 && bs != 128) ||
+        (int64_t)pages->table_ld * bs < max_seq)
+      return fail(PALU_ERR_INVALID, "page table: blocks of 16, 32, 64 or 128 and rows that hold max_seq positions");
+    p.page_table = pages->table;
+    p.table_ld = pages->table_ld;
+    p.n_blocks = pages->n_blocks;
+    while ((1 << p.blk_shift) < bs) ++p.blk_shift;
+  }
+  p.k_lat = static_cast<const __nv_bfloat16*>(k_lat);
+  p.v_lat = static_cast<const __nv_bfloat16*>(v_lat);
+  p.u_k = static_cast<const __nv_bfloat16*>(u_k);
+  p.u_v = static_cast<const __nv_bfloat16*>(u_v);
+  p.cos = cos;
+  p.sin = sin;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.tiles = reinterpret_cast<const int4*>(static_cast<const char*>(plan_data) + plan->off_tiles);
+  p.n_kv = plan->n_kv_heads;
+  p.n_groups = n_groups;
+  p.r_k = r_k;
+  p.r_v = r_v;
+  p.max_seq = max_seq;
+  p.jobs = p.n_kv + (u_v ? p.n_kv : n_groups);
+  // heads per CTA: as many as leave every SM a few CTAs (a CTA reads its tokens' table rows once)
+  const int64_t want = 8LL * device_sms();
+  int splits = (int)std::min<int64_t>(p.jobs, std::max<int64_t>(1, (want + plan->n_tiles - 1) / plan->n_tiles));
+  p.per_cta = (p.jobs + splits - 1) / splits;
+  splits = (p.jobs + p.per_cta - 1) / p.per_cta;
+  const int smem = 2 * palu::rb::stage_bytes(u_v ? std::max(r_k, r_v) : r_k) + palu::rb::kOutBytes;
+  if (cudaFuncSetAttribute(palu::rb::palu_rebuild_kv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return cuda_check("cudaFuncSetAttribute(rebuild)");
+  palu::rb::palu_rebuild_kv_kernel<<<dim3(plan->n_tiles, splits), palu::rb::kThreads, smem, stream>>>(p);
+  return cuda_check("rebuild kernel launch");
+}
+
+int palu_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t rows, int32_t vocab, const void* tokens, int32_t tokens64,
+                        int32_t top, float* logprob, float* entropy, float* top_logprob, int64_t* top_id, palu_stream_t stream) {
+  g_err.clear();
+  if (rows < 0 || vocab <= 0) return fail(PALU_ERR_INVALID, "logprobs: rows must not be negative and vocab positive (got %lld, %d)", (long long)rows, vocab);
+  if (dtype != PALU_BF16 && dtype != PALU_F32) return fail(PALU_ERR_INVALID, "logits dtype must be bf16 or f32");
+  if (top < 0 || top > palu::lp::kMaxTop || top > vocab)
+    return fail(PALU_ERR_INVALID, "top must be in [0, 32] and at most the vocabulary's %d, got %d", vocab, top);
+  if (rows > 1 && ld < vocab) return fail(PALU_ERR_INVALID, "logits rows of %lld elements cannot hold %d", (long long)ld, vocab);
+  if (rows == 0) return PALU_OK;
+  if (!logits || !tokens || !logprob || !entropy || (top > 0 && (!top_logprob || !top_id)))
+    return fail(PALU_ERR_INVALID, "logprobs: every pointer must be set");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype == PALU_F32 ? 4 : 2) != 0) return fail(PALU_ERR_INVALID, "logits are not aligned to their type");
+  const palu::lp::Params p{logits, ld, rows, vocab, top, tokens, tokens64, logprob, entropy, top_logprob, top_id};
+  // CTAs a row: enough for two per SM, as long as each has a stage of chunks or more
+  const int sms = device_sms(), per = 16 / (dtype == PALU_F32 ? 4 : 2) * palu::lp::kThreads;
+  int c = 1;
+  while (c < 8 && rows * c * 2 <= 2 * sms && vocab >= per * c * 2) c *= 2;
+  const int smem = palu::lp::kStages * palu::lp::kStageBytes;
+  auto kern = dtype == PALU_F32 ? palu::lp::palu_token_logprobs_kernel<float> : palu::lp::palu_token_logprobs_kernel<__nv_bfloat16>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return cuda_check("cudaFuncSetAttribute(logprobs)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, 3 * sms / c)) * c));
+  cfg.blockDim = dim3(palu::lp::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)c, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p) != cudaSuccess) return cuda_check("logprobs kernel launch");
+  return cuda_check("logprobs kernel launch");
+}
+
+size_t palu_page_workspace_bytes(int32_t n_blocks) { return n_blocks > 0 ? 16 + (size_t)n_blocks * 12 : 0; }
+
+int palu_reserve_pages(const palu_page_pool* pool, const int32_t* rows, const int32_t* lens, int32_t n, palu_stream_t stream) {
+  return guarded([&]() -> int {
+    palu::pg::Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (n > 0 && !lens) return fail(PALU_ERR_INVALID, "lens must hold n entries");
+    if (int st = check_rows("rows", rows, lens, n, p)) return st;
+    for (int i = 0; i < n; i += palu::pg::kMaxPairs) {
+      palu::pg::RowLens a;
+      a.n = std::min(palu::pg::kMaxPairs, n - i);
+      std::copy(rows + i, rows + i + a.n, a.row);
+      std::copy(lens + i, lens + i + a.n, a.len);
+      palu::pg::palu_reserve_pages_kernel<<<1, palu::pg::kPlanThreads, 0, stream>>>(p, a);
+      if (int st = cuda_check("reserve pages launch")) return st;
+    }
+    return PALU_OK;
+  });
+}
+
+int palu_fork_pages(const palu_page_pool* pool, const palu_page_cache* caches, int32_t n_caches, const int32_t* parents,
+                    const int32_t* children, const int32_t* lens, int32_t n, void* workspace, size_t workspace_bytes, palu_stream_t stream) {
+  return guarded([&]() -> int {
+    palu::pg::Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (int st = check_caches(caches, n_caches, p.n_pages)) return st;
+    if (n > 0 && (!lens || !parents)) return fail(PALU_ERR_INVALID, "parents and lens must hold n entries");
+    if (int st = check_rows("children", children, lens, n, p)) return st;
+    std::vector<int32_t> kids(children, children + n);
+    std::sort(kids.begin(), kids.end());
+    for (int i = 0; i < n; ++i) {
+      if (parents[i] < 0 || parents[i] >= p.rows) return fail(PALU_ERR_INVALID, "parents: row %d is outside [0, %d)", parents[i], p.rows);
+      if (std::binary_search(kids.begin(), kids.end(), parents[i]))
+        return fail(PALU_ERR_INVALID, "row %d is a parent and a child of the same fork", parents[i]);
+    }
+    if (!workspace || workspace_bytes < palu_page_workspace_bytes(p.n_pages) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+      return fail(PALU_ERR_WORKSPACE, "page workspace of %zu bytes (16-byte aligned) needed", palu_page_workspace_bytes(p.n_pages));
+    const palu::pg::Moves mv{static_cast<int32_t*>(workspace), reinterpret_cast<int2*>(static_cast<char*>(workspace) + 16)};
+    for (int i = 0; i < n; i += palu::pg::kMaxPairs) {
+      palu::pg::ForkList a;
+      a.n = std::min(palu::pg::kMaxPairs, n - i);
+      int copies = 0;
+      for (int x = 0; x < a.n; ++x) {
+        a.parent[x] = parents[i + x];
+        a.child[x] = children[i + x];
+        a.len[x] = lens[i + x];
+        copies += lens[i + x] % p.page_size != 0;
+      }
+      palu::pg::palu_fork_pages_kernel<<<1, palu::pg::kPlanThreads, 0, stream>>>(p, mv, a);
+      if (int st = cuda_check("fork pages launch")) return st;
+      if (copies > 0)
+        if (int st = apply_moves(p, mv, nullptr, caches, n_caches, copies, stream)) return st;
+    }
+    return PALU_OK;
+  });
+}
+
+int palu_free_pages(const palu_page_pool* pool, const int32_t* rows, int32_t n, palu_stream_t stream) {
+  return guarded([&]() -> int {
+    palu::pg::Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (int st = check_rows("rows", rows, nullptr, n, p)) return st;
+    for (int i = 0; i < n; i += palu::pg::kMaxPairs) {
+      palu::pg::RowList a;
+      a.n = std::min(palu::pg::kMaxPairs, n - i);
+      std::copy(rows + i, rows + i + a.n, a.row);
+      palu::pg::palu_free_pages_kernel<<<a.n, 256, 0, stream>>>(p, a);
+      if (int st = cuda_check("free pages launch")) return st;
+    }
+    return PALU_OK;
+  });
+}
+
+int palu_compact_pages(const palu_page_pool* pool, const palu_page_cache* caches, int32_t n_caches, void* workspace,
+                       size_t workspace_bytes, palu_stream_t stream) {
+  return guarded([&]() -> int {
+    palu::pg::Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (int st = check_caches(caches, n_caches, p.n_pages)) return st;
+    if (!workspace || workspace_bytes < palu_page_workspace_bytes(p.n_pages) || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+      return fail(PALU_ERR_WORKSPACE, "page workspace of %zu bytes (16-byte aligned) needed", palu_page_workspace_bytes(p.n_pages));
+    const palu::pg::Moves mv{static_cast<int32_t*>(workspace), reinterpret_cast<int2*>(static_cast<char*>(workspace) + 16)};
+    int32_t* target = reinterpret_cast<int32_t*>(mv.list + p.n_pages);
+    palu::pg::palu_compact_pages_kernel<<<1, palu::pg::kPlanThreads, 0, stream>>>(p, mv, target);
+    if (int st = cuda_check("compact pages launch")) return st;
+    return apply_moves(p, mv, target, caches, n_caches, p.n_pages / 2 + 1, stream);
+  });
+}
+
+int palu_copy_pages(const palu_page_cache* caches, int32_t n_caches, int32_t n_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    palu_stream_t stream) {
+  return guarded([&]() -> int {
+    if (n_blocks <= 0) return fail(PALU_ERR_INVALID, "n_blocks must be positive, got %d", n_blocks);
+    if (int st = check_caches(caches, n_caches, n_blocks)) return st;
+    if (n < 0 || (n > 0 && (!src || !dst))) return fail(PALU_ERR_INVALID, "src and dst must hold n entries");
+    for (int i = 0; i < n; ++i)
+      if (src[i] < 0 || src[i] >= n_blocks || dst[i] < 0 || dst[i] >= n_blocks)
+        return fail(PALU_ERR_INVALID, "copy %d -> %d is outside [0, %d)", src[i], dst[i], n_blocks);
+    std::vector<int32_t> to(dst, dst + n);
+    std::sort(to.begin(), to.end());
+    for (int i = 1; i < n; ++i)
+      if (to[i] == to[i - 1]) return fail(PALU_ERR_INVALID, "block %d is copied to twice", to[i]);
+    for (int i = 0; i < n; ++i)
+      if (src[i] != dst[i] && std::binary_search(to.begin(), to.end(), src[i]))
+        return fail(PALU_ERR_INVALID, "block %d is copied from and copied to by the same call", src[i]);
+    for (int i = 0; i < n; i += palu::pg::kMaxCopies) {
+      palu::pg::CopyList l;
+      l.n = std::min(palu::pg::kMaxCopies, n - i);
+      for (int x = 0; x < l.n; ++x) l.move[x] = make_int2(src[i + x], dst[i + x]);
+      for (int c = 0; c < n_caches; c += palu::pg::kMaxCaches) {
+        palu::pg::Caches a;
+        int64_t most;
+        const int m = std::min(palu::pg::kMaxCaches, n_caches - c);
+        const bool wide = fill_caches(caches + c, m, a, most);
+        const dim3 grid(copy_grid(m, l.n, most), m);
+        if (wide) palu::pg::palu_copy_pages_kernel<uint4><<<grid, palu::pg::kCopyThreads, 0, stream>>>(n_blocks, l, a);
+        else palu::pg::palu_copy_pages_kernel<uint8_t><<<grid, palu::pg::kCopyThreads, 0, stream>>>(n_blocks, l, a);
+        if (int st = cuda_check("copy pages launch")) return st;
+      }
+    }
+    return PALU_OK;
+  });
 }
 
 }  // extern "C"

@@ -26,6 +26,8 @@ EXPORTED = ("palu_decode_attn", "palu_decode_attn_static", "palu_decode_attn_pag
             "palu_set_wait_limit", "palu_decode_attn_f8", "palu_quantize_latents_f8", "palu_append_latents_f8",
             "palu_decode_attn_f4", "palu_quantize_latents_f4", "palu_append_latents_f4",
             "palu_plan_prefill", "palu_prefill_workspace_bytes", "palu_prefill_attn",
+            "palu_rebuild_kv", "palu_token_logprobs", "palu_page_workspace_bytes", "palu_reserve_pages",
+            "palu_fork_pages", "palu_free_pages", "palu_compact_pages", "palu_copy_pages",
             "palu_last_error", "palu_version")
 PALU_KERNEL_AUTO, PALU_KERNEL_MMA, PALU_KERNEL_TC = 0, 1, 2
 PALU_ROPE_ABSOLUTE, PALU_ROPE_CHUNK_RELATIVE = 0, 1
@@ -46,7 +48,16 @@ class PrefillPlanInfo(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_int64) for n in ("bytes", "q_tokens", "k_tokens", "off_start", "off_pieces", "off_merges",
                                                "off_tiles")]
                 + [(n, ctypes.c_int32) for n in ("n_seq", "n_q_heads", "n_kv_heads", "pos_per_chain", "n_ctas", "n_pieces",
-                                                 "n_merges", "n_slots", "n_tiles")])
+                                                 "n_merges", "n_slots", "n_tiles", "max_k_len", "max_row")])
+
+
+class PagePoolInfo(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("table", "refs", "mapped", "status")]
+                + [(n, ctypes.c_int32) for n in ("rows", "blocks_per_row", "n_blocks", "block_size")])
+
+
+class PageCache(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("block_stride", ctypes.c_int64), ("block_bytes", ctypes.c_int64)]
 
 
 _lib = None
@@ -118,6 +129,20 @@ def load() -> ctypes.CDLL:
     lib.palu_prefill_workspace_bytes.restype = sz
     lib.palu_prefill_attn.argtypes = [vp, i64, i64, vp, i64, i64, vp, i64, i64, vp, i32, plan_p, vp, vp, sz, f32, vp]
     lib.palu_prefill_attn.restype = ctypes.c_int
+    lib.palu_rebuild_kv.argtypes = [vp, vp, vp, vp, vp, vp, pages_p, plan_p, vp, vp, vp, i32, i32, i32, i32, vp]
+    lib.palu_rebuild_kv.restype = ctypes.c_int
+    lib.palu_token_logprobs.argtypes = [vp, i64, i32, i64, i32, vp, i32, i32, vp, vp, vp, vp, vp]
+    lib.palu_token_logprobs.restype = ctypes.c_int
+    pool_p, cache_p = ctypes.POINTER(PagePoolInfo), ctypes.POINTER(PageCache)
+    lib.palu_page_workspace_bytes.argtypes = [i32]
+    lib.palu_page_workspace_bytes.restype = sz
+    lib.palu_reserve_pages.argtypes = [pool_p, i32_p, i32_p, i32, vp]
+    lib.palu_fork_pages.argtypes = [pool_p, cache_p, i32, i32_p, i32_p, i32_p, i32, vp, sz, vp]
+    lib.palu_free_pages.argtypes = [pool_p, i32_p, i32, vp]
+    lib.palu_compact_pages.argtypes = [pool_p, cache_p, i32, vp, sz, vp]
+    lib.palu_copy_pages.argtypes = [cache_p, i32, i32, i32_p, i32_p, i32, vp]
+    for f in ("reserve", "fork", "free", "compact", "copy"):
+        getattr(lib, f"palu_{f}_pages").restype = ctypes.c_int
     lib.palu_last_error.argtypes = []
     lib.palu_last_error.restype = ctypes.c_char_p
     lib.palu_version.argtypes = []

@@ -1,9 +1,9 @@
-"""Prefill of packed prompts: the batch's plan and the causal attention over it.
+"""Prefill of packed prompts: the batch's plan, the causal attention over it, and the keys and values of a cached prefix.
 
 A packed batch holds sequences of different lengths one after another, without padding: sequence s has ``q_lens[s]``
 query positions and ``k_lens[s]`` keys, its last query aligned with its last key (a prompt: equal lengths; a prompt
 chunk behind a cached prefix: more keys than queries). ``PrefillPlan`` lays the batch's work out once, on the host;
-every layer of a forward pass then uses it (``prefill_attn``). The reference prefills one user's padded prompt at a
+every layer of a forward pass then uses it (``rebuild_kv``, ``prefill_attn``). The reference prefills one user's padded prompt at a
 time with the stock attention op (palu_tt/attention.py:382-516).
 """
 from __future__ import annotations
@@ -139,3 +139,58 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Prefil
         v.stride(1), out.data_ptr(), d_v, plan.info_ptr, plan.data.data_ptr(), _lib.ptr(ws), need,
         HEAD_DIM ** -0.5 if scale is None else float(scale), stream))
     return out
+
+
+def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+               plan: PrefillPlan, *, u_v: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None):
+    """The packed keys and values of the plan's ``k_lens`` cached positions per sequence (palu_rebuild_kv), which
+    ``prefill_attn`` takes: K = R_pos(latent U_k) [k_tokens, n_kv, 128] and V = latent U_v [k_tokens, n_kv, 128], or the V
+    latents themselves [k_tokens, n_groups, r_v] without ``u_v`` (absorbed V).
+
+    k_latent / v_latent: bf16 caches [B, n_groups, S, r], or paged [n_blocks, n_groups, block_size, r] with ``page_table``
+    [rows, blocks per row] int32 (an entry outside the cache reads as zero latents); u_k [n_kv, r_k, 128], u_v [n_kv, r_v,
+    128] bf16; cos / sin [>= longest k_len, 128] fp32 as the layer's tables. Sequence s reads cache row ``plan.rows[s]``.
+    fp32 accumulation and rotation, one rounding to bf16."""
+    _lib.require_cuda(k_latent, v_latent, u_k, cos, sin, u_v, page_table)
+    for t, what in ((k_latent, "k_latent"), (v_latent, "v_latent"), (u_k, "u_k"), (cos, "cos"), (sin, "sin"), (u_v, "u_v"),
+                    (page_table, "page_table")):
+        if t is not None and t.device != plan.device:
+            raise RuntimeError(f"{what} is on {t.device}, the plan on {plan.device}")
+    for t, what in ((k_latent, "k_latent"), (v_latent, "v_latent"), (u_k, "u_k"), (u_v, "u_v")):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise RuntimeError(f"{what} must be bf16, got {t.dtype}")
+    if k_latent.dim() != 4 or v_latent.dim() != 4 or k_latent.shape[:3] != v_latent.shape[:3]:
+        raise RuntimeError(f"k_latent and v_latent must be [B, n_groups, S, r] with the same leading dims, got "
+                           f"{tuple(k_latent.shape)} and {tuple(v_latent.shape)}")
+    n_groups, S, r_k, r_v = k_latent.shape[1], k_latent.shape[2], k_latent.shape[3], v_latent.shape[3]
+    n_kv = plan.n_kv_heads
+    if tuple(u_k.shape) != (n_kv, r_k, HEAD_DIM):
+        raise RuntimeError(f"u_k must be [{n_kv}, {r_k}, 128], got {tuple(u_k.shape)}")
+    if u_v is not None and tuple(u_v.shape) != (n_kv, r_v, HEAD_DIM):
+        raise RuntimeError(f"u_v must be [{n_kv}, {r_v}, 128], got {tuple(u_v.shape)}")
+    longest, last_row = int(plan.info.max_k_len), int(plan.info.max_row)
+    for t, what in ((cos, "cos"), (sin, "sin")):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != HEAD_DIM or t.shape[0] < longest or not t.is_contiguous():
+            raise RuntimeError(f"{what} must be a contiguous fp32 [>= {longest}, 128] table, got {t.dtype} {tuple(t.shape)}")
+    rows, pg = k_latent.shape[0], None
+    if page_table is not None:
+        page_table = page_table.to(torch.int32)
+        page_table = page_table if page_table.stride(-1) == 1 else page_table.contiguous()
+        rows, S = page_table.shape[0], page_table.shape[1] * k_latent.shape[2]
+        pg = ctypes.byref(_lib.pages(page_table, k_latent.shape[2], k_latent.shape[0]))
+    if longest > S or last_row >= rows:
+        raise RuntimeError(f"the plan's longest sequence ({longest}) and last cache row ({last_row}) must fit the {rows} rows of "
+                           f"{S} positions")
+    if k_latent.device.index != torch.cuda.current_device():
+        with torch.cuda.device(k_latent.device):
+            return rebuild_kv(k_latent, v_latent, u_k, cos, sin, plan, u_v=u_v, page_table=page_table)
+    k_latent, v_latent, u_k = k_latent.contiguous(), v_latent.contiguous(), u_k.contiguous()
+    u_v = u_v.contiguous() if u_v is not None else None
+    k = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=k_latent.device)
+    v = torch.empty(plan.k_tokens, *((n_kv, HEAD_DIM) if u_v is not None else (n_groups, r_v)), dtype=torch.bfloat16, device=k.device)
+    stream = _lib.stream_handle(k.device)
+    plan.use_on(stream)
+    _lib.check(_lib.load().palu_rebuild_kv(
+        k_latent.data_ptr(), v_latent.data_ptr(), u_k.data_ptr(), _lib.ptr(u_v), cos.data_ptr(), sin.data_ptr(), pg,
+        plan.info_ptr, plan.data.data_ptr(), k.data_ptr(), v.data_ptr(), n_groups, r_k, r_v, S, stream))
+    return k, v

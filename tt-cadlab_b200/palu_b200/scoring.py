@@ -1,0 +1,58 @@
+"""Log probabilities of given tokens, the entropy and the top alternatives of rows of logits.
+
+What a server answers next to its tokens, and what scores a prompt (perplexity, the quality measure of a compressed
+cache): one kernel over the logits as the LM head wrote them (bf16 or fp32), without an fp32 copy, a softmax or a sort.
+The reference decodes greedily and has none of this (palu_tt/generate.py:53-62).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from palu_b200 import _lib
+
+MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """``logprob`` [N] of the given tokens and ``entropy`` [N] of the rows (nats, fp32); ``top_logprob`` [N, k] fp32 and
+    ``top_id`` [N, k] int64, highest first."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor
+    top_id: torch.Tensor
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Per row of ``logits`` [N, vocab] (bf16 or fp32, rows of any stride): the log probability of ``tokens`` [N] (int64 or
+    int32), the entropy, and the ``top`` (at most 32) highest log probabilities with their ids (palu_token_logprobs).
+
+    Equal logits are ordered by the lower id. A negative token stands for none and gives 0; one at or past the vocabulary
+    gives NaN. A logit of -inf has probability 0; a row of -inf only, or with a NaN or +inf in it, has no distribution:
+    its log probabilities and entropy are NaN. Everything is computed in fp32."""
+    _lib.require_cuda(logits, tokens)
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.shape[1] < 1:
+        raise RuntimeError(f"logits must be bf16 or fp32 [N, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    n, vocab = logits.shape
+    if tuple(tokens.shape) != (n,) or tokens.dtype not in (torch.int64, torch.int32):
+        raise RuntimeError(f"tokens must be [{n}] int64 or int32, got {tokens.dtype} {tuple(tokens.shape)}")
+    if tokens.device != logits.device:
+        raise RuntimeError(f"tokens are on {tokens.device}, logits on {logits.device}")
+    top = int(top)
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise RuntimeError(f"top must be in [0, {min(MAX_TOP, vocab)}] (at most 32, at most the vocabulary), got {top}")
+    if logits.device.index != torch.cuda.current_device():
+        with torch.cuda.device(logits.device):
+            return token_logprobs(logits, tokens, top)
+    if logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab):
+        logits = logits.contiguous()
+    tokens = tokens.contiguous()
+    f32 = torch.empty(n * (2 + top), dtype=torch.float32, device=logits.device)
+    lp, ent, tv = f32[:n], f32[n:2 * n], f32[2 * n:].view(n, top)
+    ti = torch.empty(n, top, dtype=torch.int64, device=logits.device)
+    _lib.check(_lib.load().palu_token_logprobs(
+        logits.data_ptr(), logits.stride(0), _lib.PALU_F32 if logits.dtype == torch.float32 else _lib.PALU_BF16, n, vocab,
+        tokens.data_ptr(), int(tokens.dtype == torch.int64), top, lp.data_ptr(), ent.data_ptr(), tv.data_ptr(), ti.data_ptr(),
+        _lib.stream_handle(logits.device)))
+    return TokenLogprobs(lp, ent, tv, ti)
