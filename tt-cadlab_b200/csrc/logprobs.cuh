@@ -11,6 +11,12 @@
 // of the CTA's slice: it copies them into its own ring in shared memory (cp.async, so loads run ahead of the arithmetic
 // and into the next row) and keeps its own (maximum, R, T) until the slice is done.
 //
+// Per element that is an exponential (16 a clock and SM: 1051 MB of bf16 keep them busy for 3/4 of the time that reading
+// takes) and about six more instructions, so the loop has no branch that data takes often: the maximum is kept out of
+// R by a comparator per element, which passes the larger one on and hands the smaller one to the sum (on pairs of bf16
+// at once), and the sums refer to a value that moves only when the maximum outgrows it by e^60. (With the exact running
+// maximum as reference, every chunk in which one of a warp's 32 maxima grew took a slow path: 4096 x 128256 took 600 us.)
+//
 // Top k: elements are ordered by value, NaN highest, equal ones by the lower index; as one 64-bit key per element all
 // keys differ. With t the k-th largest of the threads' maxima, every element of the top k is at least t and belongs to
 // one of the k threads whose maximum is at least t: only the elements of those are looked at again (about k / 256 of the
@@ -96,79 +102,165 @@ PALU_DEVINL void widen(const uint4& w, float (&x)[4]) {  // 4 fp32
   x[2] = __uint_as_float(w.z);
   x[3] = __uint_as_float(w.w);
 }
+// Two bf16 at a time; NaN wins a maximum and loses a minimum.
+PALU_DEVINL uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+PALU_DEVINL uint32_t min2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 PALU_DEVINL float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-// A product of e^d and d (d <= 0, in units of log 2) in which e^-inf wins.
-constexpr float kFloor = -1000.f;
+PALU_DEVINL uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+PALU_DEVINL void un2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v)); }
+PALU_DEVINL uint64_t f2add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+PALU_DEVINL uint64_t f2mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+PALU_DEVINL uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 
-// Running (maximum, R, T = sum e^(x - m) (x - m) log2(e)) of the elements seen.
+// d = (x - ref) log2(e) is kept above this, so that an element of -inf adds e^d d = 0 and not 0 * inf.
+constexpr float kFloor = -1000.f;
+constexpr float kOutgrown = 60.f;  // sums of e^60 stay in range
+
+// The elements seen: the largest, and R and T = sum e^(x - m) (x - m) log2(e) over the others.
 struct Stat {
-  uint32_t order;  // of the maximum; 0: nothing seen
-  uint32_t index;  // its lowest index
   float m, r, t;
-  PALU_DEVINL void clear() {
-    order = 0;
-    index = 0;
-    m = -INFINITY;
-    r = t = 0.f;
-  }
-  // move the reference up to m2 (not below m); the old maximum becomes an ordinary element
-  PALU_DEVINL void raise(float m2) {
-    if (order != 0 && m != -INFINITY) {
-      const float d = (m - m2) * kLog2e, a = fast_exp2(d), all = r + 1.f;
-      t = a == 0.f ? 0.f : a * (t + all * d);
-      r = all * a;
-    } else {
-      r = t = 0.f;
-    }
-    m = m2;
-  }
-  template <int N>
-  PALU_DEVINL void add(const float (&x)[N], uint32_t first) {
-    float hi = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) hi = max_nan(hi, x[i]);
-    const uint32_t o = order_of(hi);
-    if (o > order) {  // rare after the first chunks
-      raise(hi);
-      order = o;
-      bool out = false;  // the new maximum itself stays out of R
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!out && order_of(x[i]) == o) {
-          out = true;
-          index = first + i;
-        } else if (x[i] != -INFINITY) {
-          const float d = (x[i] - m) * kLog2e, e = fast_exp2(d);
-          r += e;
-          t += e * fmaxf(d, kFloor);
-        }
-      }
-    } else if (m != -INFINITY) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float d = (x[i] - m) * kLog2e, e = fast_exp2(d);
-        r += e;
-        t += e * fmaxf(d, kFloor);
-      }
-    }
-  }
-  // join another's elements
-  PALU_DEVINL void join(const Stat& b) {
-    if (b.order == 0) return;
-    const uint64_t ka = order ? key_of(order, index) : 0, kb = key_of(b.order, b.index);
-    Stat lo = b;
-    if (kb > ka) {
-      lo = *this;
-      *this = b;
-    }
-    if (lo.order == 0 || lo.m == -INFINITY) return;
-    const float d = (lo.m - m) * kLog2e, a = fast_exp2(d), all = lo.r + 1.f;  // lo's maximum is an ordinary element here
+  PALU_DEVINL void join(const Stat& b) {  // no element: m = -inf, r = t = 0
+    const bool up = b.m > m || isnan(b.m);
+    const Stat lo = up ? *this : b;
+    if (up) *this = b;
+    if (lo.m == -INFINITY) return;  // adds nothing
+    const float d = (lo.m - m) * kLog2e, a = fast_exp2(d), all = lo.r + 1.f;  // lo's maximum is one of the others here
     r += all * a;
     if (a != 0.f) t += a * (lo.t + all * d);
+  }
+};
+
+// A thread's running sums over its elements, against a reference that is one of its early elements.
+template <typename T>
+struct Run;
+
+struct Sums {
+  float ref;
+  uint64_t r, t;  // two partial sums each
+  PALU_DEVINL void clear() {
+    ref = -INFINITY;
+    r = t = 0;
+  }
+  PALU_DEVINL void raise(float to) {
+    const float d = (ref - to) * kLog2e, a = fast_exp2(d);  // ref -inf: a = 0
+    float r0, r1, t0, t1;
+    un2(r, r0, r1);
+    un2(t, t0, t1);
+    t = a == 0.f ? 0 : f2(a * (t0 + r0 * d), a * (t1 + r1 * d));
+    r = a == 0.f ? 0 : f2(r0 * a, r1 * a);
+    ref = to;
+  }
+  PALU_DEVINL void add(float x0, float x1) {
+    float d0, d1;
+    un2(f2mul(f2add(f2(x0, x1), f2(-ref, -ref)), f2(kLog2e, kLog2e)), d0, d1);
+    d0 = fmaxf(d0, kFloor);  // also for NaN, whose row is NaN by its maximum
+    d1 = fmaxf(d1, kFloor);
+    const uint64_t e = f2(fast_exp2(d0), fast_exp2(d1));
+    r = f2add(r, e);
+    t = f2fma(e, f2(d0, d1), t);
+  }
+  // the sums of everything but the maximum m, against m
+  PALU_DEVINL Stat stat(float m) const {
+    float r0, r1, t0, t1;
+    un2(r, r0, r1);
+    un2(t, t0, t1);
+    Stat s{m, 0.f, 0.f};
+    if (m == -INFINITY) return s;
+    const float d = (m - ref) * kLog2e, a = fast_exp2(-d);
+    s.r = (r0 + r1) * a;
+    s.t = ((t0 + t1) - d * (r0 + r1)) * a;
+    return s;
+  }
+};
+
+template <>
+struct Run<float> {
+  Sums s;
+  float m;
+  int at;  // the chunk that brought m
+  PALU_DEVINL void clear() {
+    s.clear();
+    m = -INFINITY;
+    at = -1;
+  }
+  PALU_DEVINL void add(const uint4& w, int chunk) {
+    const float x0 = __uint_as_float(w.x), x1 = __uint_as_float(w.y), x2 = __uint_as_float(w.z), x3 = __uint_as_float(w.w);
+    const float a = max_nan(x0, x1), b = max_nan(x2, x3), c = max_nan(a, b);
+    const float before = m;
+    m = max_nan(m, c);
+    if (c > s.ref + kOutgrown) s.raise(c);
+    if (__float_as_uint(m) != __float_as_uint(before) || at < 0) at = chunk;
+    s.add(fminf(x0, x1), fminf(x2, x3));
+    s.add(fminf(a, b), fminf(before, c));
+  }
+  PALU_DEVINL float max() const { return m; }
+  PALU_DEVINL int chunk(float) const { return at; }
+  PALU_DEVINL Stat stat() const { return s.stat(m); }
+};
+template <>
+struct Run<__nv_bfloat16> {
+  Sums s;
+  uint32_t m;      // the maxima of the even and of the odd elements
+  int at0, at1;    // the chunks that brought them
+  PALU_DEVINL void clear() {
+    s.clear();
+    m = 0xFF80FF80u;
+    at0 = at1 = -1;
+  }
+  static PALU_DEVINL float low(uint32_t w) { return __uint_as_float(w << 16); }
+  static PALU_DEVINL float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+  PALU_DEVINL void add(const uint4& w, int chunk) {
+    const uint32_t a = max2_nan(w.x, w.y), b = max2_nan(w.z, w.w), c = max2_nan(a, b), before = m;
+    m = max2_nan(m, c);
+    const float top = max_nan(low(c), high(c));
+    if (top > s.ref + kOutgrown) s.raise(top);
+    if (m != before || at0 < 0) {
+      if ((m ^ before) & 0xFFFFu || at0 < 0) at0 = chunk;
+      if ((m ^ before) >> 16 || at1 < 0) at1 = chunk;
+    }
+    const uint32_t lo[4] = {min2(w.x, w.y), min2(w.z, w.w), min2(a, b), min2(before, c)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.add(low(lo[i]), high(lo[i]));
+  }
+  PALU_DEVINL float max() const { return max_nan(low(m), high(m)); }
+  // the chunk of the first element that equals the maximum v
+  PALU_DEVINL int chunk(float v) const {
+    const bool e0 = order_of(low(m)) == order_of(v), e1 = order_of(high(m)) == order_of(v);
+    return e0 && e1 ? min(at0, at1) : (e0 ? at0 : at1);
+  }
+  PALU_DEVINL Stat stat() const {
+    const float a = low(m), b = high(m), hi = max(), lo = fminf(a, b);
+    Sums all = s;
+    all.add(lo, -INFINITY);
+    return all.stat(hi);
   }
 };
 
@@ -198,6 +290,26 @@ PALU_DEVINL float load1(const Params& p, int64_t row, int i) {
   const T v = static_cast<const T*>(p.logits)[row * p.ld + i];
   if constexpr (sizeof(T) == 4) return v;
   else return __bfloat162float(v);
+}
+
+// The element outside the body that goes to a CTA's thread (counted from the last), or -1.
+PALU_DEVINL int edge_element(const Slice& s, int rank, int i, int vocab) {
+  if (rank != 0) return -1;
+  if (i < s.head) return i;
+  const int t = s.tail + i - s.head;
+  return t < vocab ? t : -1;
+}
+// The 8 warps' descending lists (each also in its `mine`) into one, in warp 0.
+PALU_DEVINL uint64_t merge_lists(uint64_t (*s_keys)[32], uint64_t mine, int warp, int lane) {
+#pragma unroll
+  for (int h = kWarps / 2; h; h >>= 1) {
+    if (warp < h) {
+      mine = merge_desc(mine, s_keys[warp + h][lane], lane);
+      if (h > 1) s_keys[warp][lane] = mine;
+    }
+    __syncthreads();
+  }
+  return mine;
 }
 
 template <typename T>
@@ -246,13 +358,8 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
   for (int64_t row = first; row < p.rows; row += step) {
     const Slice sl = slice_of<T>(p, row, rank, ranks);
     const int n = sl.c1 - sl.c0;
-    Stat st;
-    st.clear();
-    if (rank == 0 && tid == 0)
-      for (int i = 0; i < sl.head; ++i) {
-        const float x[1] = {load1<T>(p, row, i)};
-        st.add(x, i);
-      }
+    Run<T> run;
+    run.clear();
     int at = 0;
     do {  // an empty slice still takes its stage of the ring
       cp_async_wait<kStages - 2>();
@@ -260,30 +367,46 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
 #pragma unroll
       for (int i = 0; i < kPerStage; ++i) {
         const int c = at + i * kThreads + tid;
-        if (c < n) {
-          float x[N];
-          widen(*reinterpret_cast<const uint4*>(buf + i * kThreads * 16), x);
-          st.add(x, sl.head + (sl.c0 + c) * N);
-        }
+        if (c < n) run.add(*reinterpret_cast<const uint4*>(buf + i * kThreads * 16), c);
       }
       copy_stage();
       stage = stage + 1 == kStages ? 0 : stage + 1;
       at += kPerStage * kThreads;
     } while (at < n);
-    if (rank == 0 && tid == 1)
-      for (int i = sl.tail; i < p.vocab; ++i) {
-        const float x[1] = {load1<T>(p, row, i)};
-        st.add(x, i);
-      }
+    // the elements before and behind the body: one each to the last threads of the first CTA
+    const int edge = edge_element(sl, rank, kThreads - 1 - tid, p.vocab);
+    Stat st = run.stat();
+    if (edge >= 0) st.join(Stat{load1<T>(p, row, edge), 0.f, 0.f});
 
     // ---- the CTA's part ----
-    const uint64_t own = st.order ? key_of(st.order, st.index) : 0;
+    // the thread's largest element as a key
+    uint64_t own = 0;
+    if (p.top > 0) {
+      const float v = run.max();
+      if (n > tid) {
+        uint32_t o = order_of(v);
+        int c = run.chunk(v), c1 = c;
+        if (o == 0x80000000u) {  // zeros: -0 gave way to a later +0, but the first of them counts
+          c = tid;
+          c1 = n - 1;
+        }
+        for (; c <= c1 && own == 0; c += kThreads) {
+          float x[N];
+          widen(*reinterpret_cast<const uint4*>(sl.body + (int64_t)(sl.c0 + c) * 16), x);
+#pragma unroll
+          for (int i = N - 1; i >= 0; --i)
+            if (order_of(x[i]) == o) own = key_of(o, (uint32_t)(sl.head + (sl.c0 + c) * N + i));
+        }
+      }
+      if (edge >= 0) {
+        const uint64_t k = key_of(order_of(load1<T>(p, row, edge)), (uint32_t)edge);
+        own = k > own ? k : own;
+      }
+    }
     Stat w = st;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
       Stat b;
-      b.order = __shfl_xor_sync(0xffffffffu, w.order, o);
-      b.index = __shfl_xor_sync(0xffffffffu, w.index, o);
       b.m = __shfl_xor_sync(0xffffffffu, w.m, o);
       b.r = __shfl_xor_sync(0xffffffffu, w.r, o);
       b.t = __shfl_xor_sync(0xffffffffu, w.t, o);
@@ -291,24 +414,27 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
     }
     if (lane == 0) s_stat[warp] = w;
     uint64_t list = 0;
-    if (p.top > 1) {
+    if (p.top > 0) {
       list = sort_desc(own, lane);
       s_keys[warp][lane] = list;
     }
     __syncthreads();
+    if (p.top > 0) list = merge_lists(s_keys, list, warp, lane);  // warp 0: the 32 largest thread maxima
     if (p.top > 1) {
-      // every warp: the 32 largest thread maxima, then the elements of the owners warp, warp + 8, ...
-      uint64_t best = s_keys[0][lane];
-#pragma unroll 1
-      for (int x = 1; x < kWarps; ++x) best = merge_desc(best, s_keys[x][lane], lane);
+      if (warp == 0) s_top[lane] = list;
+      __syncthreads();
+      // every warp: the elements of the owners warp, warp + 8, ...
+      const uint64_t best = s_top[lane];
       const uint64_t least = __shfl_sync(0xffffffffu, best, p.top - 1);  // 0: fewer threads than that hold anything
       list = 0;
       for (int x = warp; x < p.top; x += kWarps) {
         const uint64_t who = __shfl_sync(0xffffffffu, best, x);
         if (who == 0) break;
         const int id = (int)index_of(who);
-        const bool edge = id < sl.head || id >= sl.tail;
-        const int owner = edge ? (id < sl.head ? 0 : 1) : ((id - sl.head) / N - sl.c0) % kThreads;
+        int owner;
+        if (id < sl.head) owner = kThreads - 1 - id;
+        else if (id >= sl.tail) owner = kThreads - 1 - (sl.head + id - sl.tail);
+        else owner = ((id - sl.head) / N - sl.c0) % kThreads;
         auto take = [&](float v, int i, bool have) {
           uint64_t k = have ? key_of(order_of(v), (uint32_t)i) : 0;
           if (k < least) k = 0;
@@ -321,31 +447,25 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
           uint4 raw = make_uint4(0, 0, 0, 0);
           if (have) raw = *reinterpret_cast<const uint4*>(sl.body + (int64_t)(sl.c0 + mc) * 16);
           widen(raw, v);
+#pragma unroll 1
+          for (int i = 0; i < N; ++i) {
+            float vi = v[0];
 #pragma unroll
-          for (int i = 0; i < N; ++i) take(v[i], sl.head + (sl.c0 + mc) * N + i, have);
+            for (int y = 1; y < N; ++y) vi = y == i ? v[y] : vi;
+            take(vi, sl.head + (sl.c0 + mc) * N + i, have);
+          }
         }
-        if (rank == 0 && owner == 0 && sl.head > 0)
-          take(lane < sl.head ? load1<T>(p, row, lane) : 0.f, lane, lane < sl.head);
-        if (rank == 0 && owner == 1 && sl.tail < p.vocab) {
-          const bool have = sl.tail + lane < p.vocab;
-          take(have ? load1<T>(p, row, sl.tail + lane) : 0.f, sl.tail + lane, have);
-        }
+        const int e = edge_element(sl, rank, kThreads - 1 - owner, p.vocab);
+        if (e >= 0) take(load1<T>(p, row, e), e, lane == 0);
       }
-      __syncthreads();
       s_keys[warp][lane] = list;
       __syncthreads();
+      list = merge_lists(s_keys, list, warp, lane);
     }
     if (warp == 0) {
       Stat a = s_stat[0];
 #pragma unroll 1
       for (int x = 1; x < kWarps; ++x) a.join(s_stat[x]);
-      if (p.top > 1) {
-        list = s_keys[0][lane];
-#pragma unroll 1
-        for (int x = 1; x < kWarps; ++x) list = merge_desc(list, s_keys[x][lane], lane);
-      } else {
-        list = lane == 0 && a.order ? key_of(a.order, a.index) : 0;
-      }
       if (ranks > 1) {
         if (lane == 0) s_cta = a;
         s_top[lane] = list;
@@ -355,12 +475,16 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
     }
     if (ranks > 1) {
       cluster.sync();
-      if (rank == 0 && warp == 0) {
-        st = s_cta;
-        list = s_top[lane];
-        for (int x = 1; x < ranks; ++x) {
-          st.join(*cluster.map_shared_rank(&s_cta, x));
-          if (p.top > 0) list = merge_desc(list, cluster.map_shared_rank(s_top, x)[lane], lane);
+      if (rank == 0) {
+        if (p.top > 0) {  // warp x takes CTA x's list
+          list = warp < ranks ? cluster.map_shared_rank(s_top, warp)[lane] : 0;
+          s_keys[warp][lane] = list;
+          __syncthreads();
+          list = merge_lists(s_keys, list, warp, lane);
+        }
+        if (warp == 0) {
+          st = s_cta;
+          for (int x = 1; x < ranks; ++x) st.join(*cluster.map_shared_rank(&s_cta, x));
         }
       }
     }
