@@ -165,3 +165,45 @@ def test_same_bits_alone_in_a_batch_on_a_stream_and_in_a_graph(cuda):
 def test_no_rows(cuda):
     lp, ent, tv, ti = run(cuda, torch.zeros(0, 50, device=cuda), torch.zeros(0, dtype=torch.long, device=cuda), 2)
     assert lp.shape == (0,) and tv.shape == (0, 2) and ti.dtype == torch.int64
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("first", [0.0, -math.inf, -3.0, -3.0e38, -1.0e6, 7.0e5], ids=str)
+def test_rows_that_start_low_or_far_out(cuda, dtype, first):
+    """The first half of the row at one value (zero, masked, the type's lowest, beyond fp32's fine range), the rest a
+    little above it in another; a row that is one value throughout is uniform."""
+    logits = torch.full((3, 40000), first).to(cuda, dtype)
+    base = logits[0, 0].float().item()
+    step = 4.0 if abs(base) < 1e5 or math.isinf(base) else abs(base) / 64
+    logits[0, 20001::7] = (base if math.isfinite(base) else 0.0) + step
+    logits[1, 39999] = (base if math.isfinite(base) else 0.0) + 2 * step
+    logits[2, 17] = base if math.isfinite(base) else 0.0
+    check(cuda, logits, torch.tensor([20001, 39999, 17], device=cuda), 5)
+
+
+def test_the_lowest_finite_value_as_a_mask(cuda):
+    logits = torch.full((2, 30000), torch.finfo(torch.bfloat16).min, dtype=torch.bfloat16, device=cuda)
+    logits[0, [100, 29999]] = torch.tensor([1.0, 2.0], dtype=torch.bfloat16, device=cuda)
+    check(cuda, logits, torch.tensor([100, 5], device=cuda), 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 9, 17, 127, 129])
+def test_short_rows_of_minus_infinities(cuda, dtype, vocab):
+    """Rows without a whole 16-byte chunk among them: the ids are the lowest, there is no distribution."""
+    from palu_b200 import scoring
+    top = min(vocab, 32)
+    wide = torch.full((5, vocab + 3), -math.inf, device=cuda).to(dtype)
+    for logits in (wide[:, :vocab], wide[:, 3:]):
+        lp, ent, tv, ti = scoring.token_logprobs(logits, torch.zeros(5, dtype=torch.long, device=cuda), top)
+        assert torch.isnan(lp).all() and torch.isnan(ent).all() and torch.isnan(tv).all()
+        assert torch.equal(ti.cpu(), torch.arange(top).expand(5, -1))
+
+
+def test_many_equal_elements_at_the_border_of_the_top(cuda):
+    """More candidates than the kernel holds at a time: the rounds of its slow look, at several cluster sizes."""
+    for n, vocab in ((1, 128256), (200, 40003), (900, 3001)):
+        logits = torch.full((n, vocab), 1.0, device=cuda)
+        logits[:, vocab // 3] = 2.0
+        logits[n // 2, :vocab // 2] = 0.5
+        check(cuda, logits, torch.zeros(n, dtype=torch.long, device=cuda), 9)

@@ -7,7 +7,7 @@
 // the log of a sum that was rounded to 1). Everything is held in fp32.
 //
 // Bound by reading the logits once. A row is read by a cluster of 1 to 8 CTAs (few rows: more CTAs a row, joined over
-// distributed shared memory; no workspace, no atomics, one launch), each thread of which owns every 256th 16-byte chunk
+// distributed shared memory; no workspace, no atomics, one launch), each thread of which owns every 128th 16-byte chunk
 // of the CTA's slice: it copies them into its own ring in shared memory (cp.async, so loads run ahead of the arithmetic
 // and into the next row) and keeps its own (maximum, R, T) until the slice is done.
 //
@@ -18,9 +18,11 @@
 // maximum as reference, every chunk in which one of a warp's 32 maxima grew took a slow path: 4096 x 128256 took 600 us.)
 //
 // Top k: elements are ordered by value, NaN highest, equal ones by the lower index; as one 64-bit key per element all
-// keys differ. With t the k-th largest of the threads' maxima, every element of the top k is at least t and belongs to
-// one of the k threads whose maximum is at least t: only the elements of those are looked at again (about k / 256 of the
-// slice, from L2), one warp a thread, and kept in sorted lists of 32 keys, one a lane, that are merged.
+// keys differ. With t the k-th largest of the threads' maxima, every element of the top k is at least t and belongs to a
+// thread whose maximum is at least t: those look again at the stage that brought their maximum, or, where a second one of
+// their stages reaches t, at all of their chunks. (Looking at all chunks of all k threads reads 64 bytes of DRAM for
+// each, the rows in flight being more than L2 holds: 4096 x 128256 bf16 with 20 alternatives took 350 us, 180 without.)
+// What is found to be at least t is sorted in lists of 32 keys, one a lane, and merged.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -29,10 +31,13 @@
 namespace palu {
 namespace lp {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kPerStage = 4, kStages = 4;  // chunks of a thread in a stage, stages of its ring
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+// Chunks of a thread in a stage, stages of its ring, CTAs an SM. 4096 x 128256 bf16, us: 3 x 3 with 7 CTAs 186, with 8 CTAs
+// 216; 4 x 3 with 7 CTAs 210; 2 x 4 with 7 CTAs 203; 256 threads, 2 x 3 with 4 CTAs 220.
+constexpr int kPerStage = 3, kStages = 3, kCtas = 7;
 constexpr int kStageBytes = kThreads * kPerStage * 16;
 constexpr int kMaxTop = 32;
+constexpr int kCands = 9 * kThreads;  // candidates for the top that a CTA holds: what one unit a thread can bring at least
 
 struct Params {
   const void* logits;
@@ -61,25 +66,27 @@ PALU_DEVINL uint64_t key_of(uint32_t order, uint32_t index) { return (uint64_t)o
 PALU_DEVINL uint32_t index_of(uint64_t key) { return 0xFFFFFFFFu - (uint32_t)key; }
 
 // 32 keys, one a lane, into descending order.
-PALU_DEVINL uint64_t sort_desc(uint64_t v, int lane) {
+template <typename K>
+PALU_DEVINL K sort_desc(K v, int lane) {
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
     for (int j = k >> 1; j; j >>= 1) {
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, v, j);
+      const K o = __shfl_xor_sync(0xffffffffu, v, j);
       const bool high = ((lane & k) == 0) == ((lane & j) == 0);  // this lane keeps the larger one
-      v = (v > o) == high ? v : o;
+      v = high ? (v > o ? v : o) : (v > o ? o : v);
     }
   return v;
 }
 // The 32 largest of two descending lists, descending.
-PALU_DEVINL uint64_t merge_desc(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  uint64_t v = a > r ? a : r;
+template <typename K>
+PALU_DEVINL K merge_desc(K a, K b, int lane) {
+  const K r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  K v = a > r ? a : r;
 #pragma unroll
   for (int j = 16; j; j >>= 1) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, v, j);
-    v = (v > o) == ((lane & j) == 0) ? v : o;
+    const K o = __shfl_xor_sync(0xffffffffu, v, j);
+    v = (lane & j) == 0 ? (v > o ? v : o) : (v > o ? o : v);
   }
   return v;
 }
@@ -106,6 +113,11 @@ PALU_DEVINL void widen(const uint4& w, float (&x)[4]) {  // 4 fp32
 PALU_DEVINL uint32_t max2_nan(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+PALU_DEVINL uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 PALU_DEVINL uint32_t min2(uint32_t a, uint32_t b) {
@@ -140,10 +152,6 @@ PALU_DEVINL uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// d = (x - ref) log2(e) is kept above this, so that an element of -inf adds e^d d = 0 and not 0 * inf.
-constexpr float kFloor = -1000.f;
-constexpr float kOutgrown = 60.f;  // sums of e^60 stay in range
-
 // The elements seen: the largest, and R and T = sum e^(x - m) (x - m) log2(e) over the others.
 struct Stat {
   float m, r, t;
@@ -158,31 +166,66 @@ struct Stat {
   }
 };
 
-// A thread's running sums over its elements, against a reference that is one of its early elements.
-template <typename T>
-struct Run;
+// The lanes' parts as one, the same in every lane.
+PALU_DEVINL Stat warp_join(const Stat& s, int lane) {
+  const uint32_t o = order_of(s.m), hi = __reduce_max_sync(0xffffffffu, o);
+  const int first = __ffs(__ballot_sync(0xffffffffu, o == hi)) - 1;
+  Stat w{value_of(hi), s.r, s.t};
+  if (lane != first) {  // its maximum is one of the others now
+    const float d = (s.m - w.m) * kLog2e, a = s.m == -INFINITY ? 0.f : fast_exp2(d), all = s.r + 1.f;
+    w.r = a == 0.f ? 0.f : a * all;
+    w.t = a == 0.f ? 0.f : a * (s.t + all * d);
+  }
+#pragma unroll
+  for (int x = 16; x; x >>= 1) {
+    w.r += __shfl_xor_sync(0xffffffffu, w.r, x);
+    w.t += __shfl_xor_sync(0xffffffffu, w.t, x);
+  }
+  return w;
+}
 
+// A thread's sums of 2^d and 2^d d over its elements, d = x log2(e) - c in one rounding. c belongs to a reference, the
+// thread's first maximum; it moves when the maximum outgrows it by kOutgrown, so that the sums stay in range. The same d
+// of the row's maximum is subtracted at the end, which takes c's own rounding out again. Elements are held above kLowest
+// (-inf: 2^d d is 0, not 0 * inf). Where the reference is so large that c's rounding would move d by more than 1/16, d
+// is taken from the difference x - ref instead, chunk by chunk on the slow path.
+constexpr float kOutgrown = 60.f, kLowest = -1e30f, kLargeRef = 524288.f, kFloor = -1000.f;
 struct Sums {
-  float ref;
+  float ref, c;
   uint64_t r, t;  // two partial sums each
   PALU_DEVINL void clear() {
     ref = -INFINITY;
+    c = 0.f;
     r = t = 0;
   }
+  PALU_DEVINL bool large() const { return !(fabsf(ref) < kLargeRef) && ref != -INFINITY; }
+  PALU_DEVINL float scaled(float x) const { return large() ? fmaxf((x - ref) * kLog2e, kFloor) : fmaf(x, kLog2e, -c); }
   PALU_DEVINL void raise(float to) {
-    const float d = (ref - to) * kLog2e, a = fast_exp2(d);  // ref -inf: a = 0
+    const float d = scaled(to), a = ref == -INFINITY ? 0.f : fast_exp2(-d);
     float r0, r1, t0, t1;
     un2(r, r0, r1);
     un2(t, t0, t1);
-    t = a == 0.f ? 0 : f2(a * (t0 + r0 * d), a * (t1 + r1 * d));
-    r = a == 0.f ? 0 : f2(r0 * a, r1 * a);
     ref = to;
+    c = to * kLog2e;
+    const float back = scaled(to);  // of the new reference against itself: c's rounding
+    t = a == 0.f ? 0 : f2(a * (t0 - r0 * d), a * (t1 - r1 * d));
+    r = a == 0.f ? 0 : f2(r0 * a, r1 * a);
+    // against `to` exactly; now against c
+    const float k = fast_exp2(back);
+    un2(r, r0, r1);
+    un2(t, t0, t1);
+    t = f2(k * (t0 + r0 * back), k * (t1 + r1 * back));
+    r = f2(r0 * k, r1 * k);
   }
   PALU_DEVINL void add(float x0, float x1) {
     float d0, d1;
-    un2(f2mul(f2add(f2(x0, x1), f2(-ref, -ref)), f2(kLog2e, kLog2e)), d0, d1);
-    d0 = fmaxf(d0, kFloor);  // also for NaN, whose row is NaN by its maximum
-    d1 = fmaxf(d1, kFloor);
+    un2(f2fma(f2(x0, x1), f2(kLog2e, kLog2e), f2(-c, -c)), d0, d1);
+    const uint64_t e = f2(fast_exp2(d0), fast_exp2(d1));
+    r = f2add(r, e);
+    t = f2fma(e, f2(d0, d1), t);
+  }
+  PALU_DEVINL void add_slow(float x0, float x1) {
+    const float d0 = fmaxf((x0 - ref) * kLog2e, kFloor), d1 = fmaxf((x1 - ref) * kLog2e, kFloor);
     const uint64_t e = f2(fast_exp2(d0), fast_exp2(d1));
     r = f2add(r, e);
     t = f2fma(e, f2(d0, d1), t);
@@ -194,73 +237,136 @@ struct Sums {
     un2(t, t0, t1);
     Stat s{m, 0.f, 0.f};
     if (m == -INFINITY) return s;
-    const float d = (m - ref) * kLog2e, a = fast_exp2(-d);
+    const float d = scaled(m), a = fast_exp2(-d);
     s.r = (r0 + r1) * a;
     s.t = ((t0 + t1) - d * (r0 + r1)) * a;
     return s;
   }
 };
 
+// A thread's elements: their maximum, which stays out of the sums (each comparison passes the larger value on and gives
+// the smaller one to the sums).
+template <typename T>
+struct Run;
 template <>
 struct Run<float> {
   Sums s;
-  float m;
-  int at;  // the chunk that brought m
+  float m, limit;  // an element above the limit takes the slow path; -inf: every one does
   PALU_DEVINL void clear() {
     s.clear();
-    m = -INFINITY;
-    at = -1;
+    m = limit = -INFINITY;
   }
-  PALU_DEVINL void add(const uint4& w, int chunk) {
-    const float x0 = __uint_as_float(w.x), x1 = __uint_as_float(w.y), x2 = __uint_as_float(w.z), x3 = __uint_as_float(w.w);
-    const float a = max_nan(x0, x1), b = max_nan(x2, x3), c = max_nan(a, b);
-    const float before = m;
+  // M chunks; returns their maximum
+  template <int M>
+  PALU_DEVINL float add(const uint4 (&w)[M]) {
+    float c = 0.f, lo[M][4];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const float x0 = __uint_as_float(w[i].x), x1 = __uint_as_float(w[i].y), x2 = __uint_as_float(w[i].z), x3 = __uint_as_float(w[i].w);
+      const float a = max_nan(x0, x1), b = max_nan(x2, x3), ab = max_nan(a, b), before = i ? c : m;
+      lo[i][0] = fminf(x0, x1);
+      lo[i][1] = fminf(x2, x3);
+      lo[i][2] = fminf(a, b);
+      if (i) lo[i][3] = fminf(before, ab);
+      c = i ? max_nan(c, ab) : ab;
+    }
+    lo[0][3] = fminf(m, c);
     m = max_nan(m, c);
-    if (c > s.ref + kOutgrown) s.raise(c);
-    if (__float_as_uint(m) != __float_as_uint(before) || at < 0) at = chunk;
-    s.add(fminf(x0, x1), fminf(x2, x3));
-    s.add(fminf(a, b), fminf(before, c));
+    if (m > limit || limit == -INFINITY) {
+      if (m > s.ref + kOutgrown) s.raise(m);
+      limit = s.large() ? -INFINITY : s.ref + kOutgrown;
+      if (s.large()) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          s.add_slow(lo[i][0], lo[i][1]);
+          s.add_slow(lo[i][2], lo[i][3]);
+        }
+        return c;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      s.add(fmaxf(lo[i][0], kLowest), fmaxf(lo[i][1], kLowest));
+      s.add(fmaxf(lo[i][2], kLowest), fmaxf(lo[i][3], kLowest));
+    }
+    return c;
   }
   PALU_DEVINL float max() const { return m; }
-  PALU_DEVINL int chunk(float) const { return at; }
   PALU_DEVINL Stat stat() const { return s.stat(m); }
 };
 template <>
 struct Run<__nv_bfloat16> {
   Sums s;
-  uint32_t m;      // the maxima of the even and of the odd elements
-  int at0, at1;    // the chunks that brought them
+  uint32_t m, limit;  // the maxima of the even and of the odd elements; the limit for both
   PALU_DEVINL void clear() {
     s.clear();
-    m = 0xFF80FF80u;
-    at0 = at1 = -1;
+    m = limit = kNone;
   }
   static PALU_DEVINL float low(uint32_t w) { return __uint_as_float(w << 16); }
   static PALU_DEVINL float high(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-  PALU_DEVINL void add(const uint4& w, int chunk) {
-    const uint32_t a = max2_nan(w.x, w.y), b = max2_nan(w.z, w.w), c = max2_nan(a, b), before = m;
+  template <int M>
+  PALU_DEVINL float add(const uint4 (&w)[M]) {
+    uint32_t c = 0, lo[M][4];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      const uint32_t a = max2_nan(w[i].x, w[i].y), b = max2_nan(w[i].z, w[i].w), ab = max2_nan(a, b);
+      lo[i][0] = min2(w[i].x, w[i].y);
+      lo[i][1] = min2(w[i].z, w[i].w);
+      lo[i][2] = min2(a, b);
+      if (i) lo[i][3] = min2(c, ab);
+      c = i ? max2_nan(c, ab) : ab;
+    }
+    lo[0][3] = min2(m, c);
     m = max2_nan(m, c);
     const float top = max_nan(low(c), high(c));
-    if (top > s.ref + kOutgrown) s.raise(top);
-    if (m != before || at0 < 0) {
-      if ((m ^ before) & 0xFFFFu || at0 < 0) at0 = chunk;
-      if ((m ^ before) >> 16 || at1 < 0) at1 = chunk;
-    }
-    const uint32_t lo[4] = {min2(w.x, w.y), min2(w.z, w.w), min2(a, b), min2(before, c)};
+    if (max2(m, limit) != limit || limit == kNone) {
+      const float hi = max();
+      if (hi > s.ref + kOutgrown) s.raise(hi);
+      // rounded towards zero: for a negative limit that is up, by less than the 2^-7 of it that the sums have room for
+      const uint32_t l = s.large() ? kNone & 0xFFFFu : __float_as_uint(s.ref + kOutgrown) >> 16;
+      limit = l << 16 | l;
+      if (s.large()) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s.add(low(lo[i]), high(lo[i]));
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) s.add_slow(low(lo[i][y]), high(lo[i][y]));
+        return top;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint32_t l = max2(lo[i][y], kLowest2);
+        s.add(low(l), high(l));
+      }
+    return top;
   }
   PALU_DEVINL float max() const { return max_nan(low(m), high(m)); }
-  // the chunk of the first element that equals the maximum v
-  PALU_DEVINL int chunk(float v) const {
-    const bool e0 = order_of(low(m)) == order_of(v), e1 = order_of(high(m)) == order_of(v);
-    return e0 && e1 ? min(at0, at1) : (e0 ? at0 : at1);
-  }
   PALU_DEVINL Stat stat() const {
-    const float a = low(m), b = high(m), hi = max(), lo = fminf(a, b);
-    Sums all = s;
-    all.add(lo, -INFINITY);
-    return all.stat(hi);
+    const float a = low(m), b = high(m);
+    Stat x = s.stat(max());
+    x.join(Stat{a < b ? a : b, 0.f, 0.f});  // the other lane's maximum is an ordinary element
+    return x;
+  }
+  static constexpr uint32_t kNone = 0xFF80FF80u;      // -inf, twice
+  static constexpr uint32_t kLowest2 = 0xF14AF14Au;  // -1e30 rounded to bf16, twice
+};
+
+// Where a thread's largest element is: the stage that brought it, and the largest element of the other stages.
+struct Where {
+  float best, rest;
+  int stage;
+  PALU_DEVINL void clear() {
+    best = rest = -INFINITY;
+    stage = 0;
+  }
+  PALU_DEVINL void add(float top, int at) {
+    rest = fmaxf(rest, fminf(top, best));
+    if (!(top <= best)) {  // a NaN too; a thread that saw one has all its elements looked at
+      best = top;
+      stage = at;
+    }
   }
 };
 
@@ -299,8 +405,9 @@ PALU_DEVINL int edge_element(const Slice& s, int rank, int i, int vocab) {
   const int t = s.tail + i - s.head;
   return t < vocab ? t : -1;
 }
-// The 8 warps' descending lists (each also in its `mine`) into one, in warp 0.
-PALU_DEVINL uint64_t merge_lists(uint64_t (*s_keys)[32], uint64_t mine, int warp, int lane) {
+// The warps' descending lists (each also in its `mine`) into one, in warp 0.
+template <typename K>
+PALU_DEVINL K merge_lists(K (*s_keys)[32], K mine, int warp, int lane) {
 #pragma unroll
   for (int h = kWarps / 2; h; h >>= 1) {
     if (warp < h) {
@@ -313,7 +420,7 @@ PALU_DEVINL uint64_t merge_lists(uint64_t (*s_keys)[32], uint64_t mine, int warp
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kCtas) palu_token_logprobs_kernel(const Params p) {
   constexpr int N = Chunk<T>::N;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -322,169 +429,210 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ uint64_t s_keys[kWarps][32];
   __shared__ Stat s_stat[kWarps];
-  __shared__ Stat s_cta;           // this CTA's part of the row, read by the cluster's first CTA
-  __shared__ uint64_t s_top[32];
+  __shared__ Stat s_cta[2];         // this CTA's part of a row, read by the cluster's first CTA
+  __shared__ uint64_t s_top[2][32];  // and its best
+  __shared__ uint32_t s_max[kWarps][32], s_least;
+  __shared__ uint64_t s_cand[kCands];
+  __shared__ int s_who[kThreads], s_owners, s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t mine = smem_u32(ring) + tid * 16;
 
-  // the copies run kStages - 1 stages ahead of the arithmetic, over the CTA's rows one after another
+  // The copies run kStages - 1 stages ahead of the arithmetic, over the CTA's rows one after another; a row takes a stage
+  // or more.
+  constexpr int kChunks = kPerStage * kThreads;
   int64_t row_l = first;
-  int at_l = 0;  // next chunk of row_l's slice to copy, relative to c0
-  Slice sl_l;
-  if (row_l < p.rows) sl_l = slice_of<T>(p, row_l, rank, ranks);
-  int stage_l = 0;
-  auto copy_stage = [&]() {
-    if (row_l < p.rows) {
-      const int n = sl_l.c1 - sl_l.c0;
+  int left_l = 0;  // chunks of row_l's slice that are not copied yet
+  const char* src_l = nullptr;
+  auto next_slice = [&]() {
+    if (row_l >= p.rows) return;  // left_l stays at 0 or below: nothing is copied
+    const Slice s = slice_of<T>(p, row_l, rank, ranks);
+    left_l = s.c1 - s.c0;
+    src_l = s.body + ((int64_t)s.c0 + tid) * 16;
+  };
+  next_slice();
+  auto copy_stage = [&](int slot) {
+    const uint32_t dst = mine + slot * kStageBytes;
+    if (left_l >= kChunks) {
 #pragma unroll
-      for (int i = 0; i < kPerStage; ++i) {
-        const int c = at_l + i * kThreads + tid;
-        if (c < n) cp_async16(mine + stage_l * kStageBytes + i * kThreads * 16, sl_l.body + (int64_t)(sl_l.c0 + c) * 16, 16);
-      }
-      at_l += kPerStage * kThreads;
-      if (at_l >= n) {
-        at_l = 0;
-        row_l += step;
-        if (row_l < p.rows) sl_l = slice_of<T>(p, row_l, rank, ranks);
-      }
+      for (int i = 0; i < kPerStage; ++i) cp_async16(dst + i * kThreads * 16, src_l + i * kThreads * 16, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPerStage; ++i)
+        if (i * kThreads + tid < left_l) cp_async16(dst + i * kThreads * 16, src_l + i * kThreads * 16, 16);
     }
     cp_async_commit();
-    stage_l = stage_l + 1 == kStages ? 0 : stage_l + 1;
+    src_l += kChunks * 16;
+    left_l -= kChunks;
+    if (left_l <= 0) {
+      left_l = 0;
+      row_l += step;
+      next_slice();
+    }
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) copy_stage();
+  for (int s = 0; s < kStages - 1; ++s) copy_stage(s);
+  int slot = 0, par = 0;
 
-  int stage = 0;
   for (int64_t row = first; row < p.rows; row += step) {
     const Slice sl = slice_of<T>(p, row, rank, ranks);
     const int n = sl.c1 - sl.c0;
     Run<T> run;
     run.clear();
-    int at = 0;
-    do {  // an empty slice still takes its stage of the ring
+    Where where;
+    where.clear();
+    int left = n, at = 0;
+    do {
       cp_async_wait<kStages - 2>();
-      const unsigned char* buf = ring + stage * kStageBytes + tid * 16;
+      const unsigned char* buf = ring + slot * kStageBytes + tid * 16;
+      if (left >= kChunks) {
+        uint4 w[kPerStage];
 #pragma unroll
-      for (int i = 0; i < kPerStage; ++i) {
-        const int c = at + i * kThreads + tid;
-        if (c < n) run.add(*reinterpret_cast<const uint4*>(buf + i * kThreads * 16), c);
+        for (int i = 0; i < kPerStage; ++i) w[i] = *reinterpret_cast<const uint4*>(buf + i * kThreads * 16);
+        const float top = run.add(w);
+        if (p.top > 0) where.add(top, at);
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kPerStage; ++i)
+          if (i * kThreads + tid < left) {
+            const uint4 w[1] = {*reinterpret_cast<const uint4*>(buf + i * kThreads * 16)};
+            const float top = run.add(w);
+            if (p.top > 0) where.add(top, at);
+          }
       }
-      copy_stage();
-      stage = stage + 1 == kStages ? 0 : stage + 1;
-      at += kPerStage * kThreads;
-    } while (at < n);
+      left -= kChunks;
+      ++at;
+      copy_stage(slot == 0 ? kStages - 1 : slot - 1);
+      slot = slot == kStages - 1 ? 0 : slot + 1;
+    } while (left > 0);
     // the elements before and behind the body: one each to the last threads of the first CTA
     const int edge = edge_element(sl, rank, kThreads - 1 - tid, p.vocab);
     Stat st = run.stat();
     if (edge >= 0) st.join(Stat{load1<T>(p, row, edge), 0.f, 0.f});
 
     // ---- the CTA's part ----
-    // the thread's largest element as a key
-    uint64_t own = 0;
-    if (p.top > 0) {
-      const float v = run.max();
-      if (n > tid) {
-        uint32_t o = order_of(v);
-        int c = run.chunk(v), c1 = c;
-        if (o == 0x80000000u) {  // zeros: -0 gave way to a later +0, but the first of them counts
-          c = tid;
-          c1 = n - 1;
-        }
-        for (; c <= c1 && own == 0; c += kThreads) {
-          float x[N];
-          widen(*reinterpret_cast<const uint4*>(sl.body + (int64_t)(sl.c0 + c) * 16), x);
-#pragma unroll
-          for (int i = N - 1; i >= 0; --i)
-            if (order_of(x[i]) == o) own = key_of(o, (uint32_t)(sl.head + (sl.c0 + c) * N + i));
-        }
-      }
-      if (edge >= 0) {
-        const uint64_t k = key_of(order_of(load1<T>(p, row, edge)), (uint32_t)edge);
-        own = k > own ? k : own;
-      }
-    }
-    Stat w = st;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      Stat b;
-      b.m = __shfl_xor_sync(0xffffffffu, w.m, o);
-      b.r = __shfl_xor_sync(0xffffffffu, w.r, o);
-      b.t = __shfl_xor_sync(0xffffffffu, w.t, o);
-      w.join(b);
-    }
+    const Stat w = warp_join(st, lane);
     if (lane == 0) s_stat[warp] = w;
+    uint32_t own = 0;  // the thread's largest element
+    if (p.top > 0) {
+      if (n > tid) own = order_of(run.max());
+      if (edge >= 0) own = max(own, order_of(load1<T>(p, row, edge)));
+      if (p.top > 1) s_max[warp][lane] = sort_desc(own, lane);
+    }
+    if (tid == 0) s_count = s_owners = 0;
+    __syncthreads();
     uint64_t list = 0;
     if (p.top > 0) {
-      list = sort_desc(own, lane);
-      s_keys[warp][lane] = list;
-    }
-    __syncthreads();
-    if (p.top > 0) list = merge_lists(s_keys, list, warp, lane);  // warp 0: the 32 largest thread maxima
-    if (p.top > 1) {
-      if (warp == 0) s_top[lane] = list;
-      __syncthreads();
-      // every warp: the elements of the owners warp, warp + 8, ...
-      const uint64_t best = s_top[lane];
-      const uint64_t least = __shfl_sync(0xffffffffu, best, p.top - 1);  // 0: fewer threads than that hold anything
-      list = 0;
-      for (int x = warp; x < p.top; x += kWarps) {
-        const uint64_t who = __shfl_sync(0xffffffffu, best, x);
-        if (who == 0) break;
-        const int id = (int)index_of(who);
-        int owner;
-        if (id < sl.head) owner = kThreads - 1 - id;
-        else if (id >= sl.tail) owner = kThreads - 1 - (sl.head + id - sl.tail);
-        else owner = ((id - sl.head) / N - sl.c0) % kThreads;
-        auto take = [&](float v, int i, bool have) {
-          uint64_t k = have ? key_of(order_of(v), (uint32_t)i) : 0;
-          if (k < least) k = 0;
-          if (__any_sync(0xffffffffu, k != 0)) list = merge_desc(list, sort_desc(k, lane), lane);
-        };
-        for (int c = owner; c < n; c += 32 * kThreads) {
-          const int mc = c + lane * kThreads;
-          const bool have = mc < n;
-          float v[N];
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (have) raw = *reinterpret_cast<const uint4*>(sl.body + (int64_t)(sl.c0 + mc) * 16);
-          widen(raw, v);
-#pragma unroll 1
-          for (int i = 0; i < N; ++i) {
-            float vi = v[0];
+      uint32_t least;  // the top-th largest of the threads' maxima; 0: fewer threads than that hold anything
+      if (p.top == 1) {
+        least = order_of(s_stat[0].m);
 #pragma unroll
-            for (int y = 1; y < N; ++y) vi = y == i ? v[y] : vi;
-            take(vi, sl.head + (sl.c0 + mc) * N + i, have);
+        for (int x = 1; x < kWarps; ++x) least = max(least, order_of(s_stat[x].m));
+      } else {
+        const uint32_t best = merge_lists(s_max, s_max[warp][lane], warp, lane);
+        if (warp == 0 && lane == p.top - 1) s_least = best;
+        __syncthreads();
+        least = s_least;
+      }
+      // The elements of at least `least` go to the candidates. A thread whose maximum is that large looks through the stage
+      // that brought it; where its other stages may hold such elements too, all threads look through its chunks. If the
+      // candidates are more than fit (many equal elements), that is done over in rounds that fit, with a merge behind each.
+      const int per = (n + kThreads - 1) / kThreads;  // chunks of a thread, at most
+      const float floor_value = value_of(least);
+      uint64_t last = 0;  // the list's top-th key: smaller ones are of no use
+      auto push = [&](float v, int i) {
+        const uint32_t o = order_of(v);
+        const uint64_t k = key_of(o, (uint32_t)i);
+        if (o >= least && k > last) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kCands) s_cand[at] = k;
+        }
+      };
+      auto look = [&](int owner, int j) {  // unit j of an owner's
+        const int c = owner + j * kThreads;
+        if (c < n) {
+          float v[N];
+          widen(*reinterpret_cast<const uint4*>(sl.body + (int64_t)(sl.c0 + c) * 16), v);
+          float hi = v[0];
+#pragma unroll
+          for (int i = 1; i < N; ++i) hi = max_nan(hi, v[i]);
+          if (!(hi < floor_value)) {  // also where one of them is NaN
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (!(v[i] < floor_value)) push(v[i], sl.head + (sl.c0 + c) * N + i);
           }
         }
-        const int e = edge_element(sl, rank, kThreads - 1 - owner, p.vocab);
-        if (e >= 0) take(load1<T>(p, row, e), e, lane == 0);
+      };
+      auto merge = [&](int have) {
+        for (int x = warp * 32; x < have; x += kThreads) {
+          const uint64_t k = x + lane < have ? s_cand[x + lane] : 0;
+          list = merge_desc(list, sort_desc(k, lane), lane);
+        }
+        s_keys[warp][lane] = list;
+        __syncthreads();
+        list = merge_lists(s_keys, list, warp, lane);
+      };
+      if (own != 0 && own >= least) {
+        if (n > tid) {  // it has a chunk
+          if (order_of(where.rest) >= least || isnan(where.best)) {
+            s_who[atomicAdd(&s_owners, 1)] = tid;
+          } else {
+#pragma unroll
+            for (int i = 0; i < kPerStage; ++i) look(tid, where.stage * kPerStage + i);
+          }
+        }
+        if (edge >= 0) push(load1<T>(p, row, edge), edge);
       }
-      s_keys[warp][lane] = list;
       __syncthreads();
-      list = merge_lists(s_keys, list, warp, lane);
+      const int count = s_owners;
+      if (count > 0) {
+        for (int who = tid / per, j = tid % per; who < count;) {
+          look(s_who[who], j);
+          for (j += kThreads; j >= per; j -= per) ++who;
+        }
+        __syncthreads();
+      }
+      if (s_count <= kCands) {
+        merge(s_count);
+      } else {
+        // every thread's chunks; then the edge elements, one more unit each
+        const int64_t units = (int64_t)kThreads * (per + 1);
+        for (int64_t u0 = 0; u0 < units; u0 += kThreads) {
+          __syncthreads();
+          if (tid == 0) s_count = 0;
+          __syncthreads();
+          const int j = (int)(u0 / kThreads);
+          if (j < per) look(tid, j);
+          else if (edge >= 0) push(load1<T>(p, row, edge), edge);
+          __syncthreads();
+          merge(s_count);
+          if (warp == 0) s_top[par][lane] = list;
+          __syncthreads();
+          last = s_top[par][p.top - 1];
+          if (warp != 0) list = 0;
+        }
+      }
     }
     if (warp == 0) {
-      Stat a = s_stat[0];
-#pragma unroll 1
-      for (int x = 1; x < kWarps; ++x) a.join(s_stat[x]);
+      st = lane < kWarps ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
+      st = warp_join(st, lane);
       if (ranks > 1) {
-        if (lane == 0) s_cta = a;
-        s_top[lane] = list;
-      } else {
-        st = a;
+        if (lane == 0) s_cta[par] = st;
+        s_top[par][lane] = list;
       }
     }
     if (ranks > 1) {
       cluster.sync();
       if (rank == 0) {
-        if (p.top > 0) {  // warp x takes CTA x's list
-          list = warp < ranks ? cluster.map_shared_rank(s_top, warp)[lane] : 0;
+        if (p.top > 0) {  // warp x takes the lists of the CTAs x, x + kWarps, ...
+          list = 0;
+          for (int x = warp; x < ranks; x += kWarps) list = merge_desc(list, cluster.map_shared_rank(s_top[par], x)[lane], lane);
           s_keys[warp][lane] = list;
           __syncthreads();
           list = merge_lists(s_keys, list, warp, lane);
         }
         if (warp == 0) {
-          st = s_cta;
-          for (int x = 1; x < ranks; ++x) st.join(*cluster.map_shared_rank(&s_cta, x));
+          st = lane < ranks ? *cluster.map_shared_rank(&s_cta[par], lane) : Stat{-INFINITY, 0.f, 0.f};
+          st = warp_join(st, lane);
         }
       }
     }
@@ -504,9 +652,10 @@ __global__ void __launch_bounds__(kThreads, 3) palu_token_logprobs_kernel(const 
         p.top_id[row * p.top + lane] = index_of(list);
       }
     }
-    if (ranks > 1) cluster.sync();  // the others' parts have been read
-    else __syncthreads();
+    par ^= 1;  // the next row's parts go to the other place; the one after that comes behind the next cluster.sync
+    __syncthreads();
   }
+  if (ranks > 1) cluster.sync();  // the first CTA has read the others' parts
 }
 
 }  // namespace lp

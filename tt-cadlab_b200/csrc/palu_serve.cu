@@ -452,16 +452,18 @@ int palu_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t r
     return fail(PALU_ERR_INVALID, "logprobs: every pointer must be set");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == PALU_F32 ? 4 : 2) != 0) return fail(PALU_ERR_INVALID, "logits are not aligned to their type");
   const palu::lp::Params p{logits, ld, rows, vocab, top, tokens, tokens64, logprob, entropy, top_logprob, top_id};
-  // CTAs a row: enough for two per SM, as long as each has a stage of chunks or more
-  const int sms = device_sms(), per = 16 / (dtype == PALU_F32 ? 4 : 2) * palu::lp::kThreads;
+  // CTAs a row (a cluster) while there are few rows. In a graph, us, with 1 / 2 / 4 / 8 a row (top 1): 1 x 128256 bf16 20 / 14 /
+  // 11 / 10, 129 x 128256 21 / 16 / 15 / 22, 300 x 128256 28 / 24 / 30 / 43, 600 x 128256 40 / 41 / 57 / 89: worth it up to
+  // about 4.3 CTAs an SM, and as long as a thread has 16 elements.
+  const int slots = palu::lp::kCtas * device_sms();
   int c = 1;
-  while (c < 8 && rows * c * 2 <= 2 * sms && vocab >= per * c * 2) c *= 2;
+  while (c < 8 && rows * c * 2 * 3 <= 13 * device_sms() && vocab >= palu::lp::kThreads * 16 * c * 2) c *= 2;
   const int smem = palu::lp::kStages * palu::lp::kStageBytes;
   auto kern = dtype == PALU_F32 ? palu::lp::palu_token_logprobs_kernel<float> : palu::lp::palu_token_logprobs_kernel<__nv_bfloat16>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return cuda_check("cudaFuncSetAttribute(logprobs)");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, 3 * sms / c)) * c));
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, slots / c)) * c));
   cfg.blockDim = dim3(palu::lp::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

@@ -48,9 +48,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab):
         logits = logits.contiguous()
     tokens = tokens.contiguous()
-    f32 = torch.empty(n * (2 + top), dtype=torch.float32, device=logits.device)
-    lp, ent, tv = f32[:n], f32[n:2 * n], f32[2 * n:].view(n, top)
-    ti = torch.empty(n, top, dtype=torch.int64, device=logits.device)
+    dev, f32 = logits.device, torch.float32
+    lp, ent = torch.empty(n, dtype=f32, device=dev), torch.empty(n, dtype=f32, device=dev)
+    tv, ti = torch.empty(n, top, dtype=f32, device=dev), torch.empty(n, top, dtype=torch.int64, device=dev)
     _lib.check(_lib.load().palu_token_logprobs(
         logits.data_ptr(), logits.stride(0), _lib.PALU_F32 if logits.dtype == torch.float32 else _lib.PALU_BF16, n, vocab,
         tokens.data_ptr(), int(tokens.dtype == torch.int64), top, lp.data_ptr(), ent.data_ptr(), tv.data_ptr(), ti.data_ptr(),
