@@ -426,16 +426,17 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.r_k = r_k;
   p.r_v = r_v;
   p.max_seq = max_seq;
-  p.jobs = p.n_kv + (u_v ? p.n_kv : n_groups);
+  p.jobs = u_v ? 2 * p.n_kv : p.n_kv;
   // heads per CTA: as many as leave every SM a few CTAs (a CTA reads its tokens' table rows once)
   const int64_t want = 8LL * device_sms();
-  int splits = (int)std::min<int64_t>(p.jobs, std::max<int64_t>(1, (want + plan->n_tiles - 1) / plan->n_tiles));
-  p.per_cta = (p.jobs + splits - 1) / splits;
-  splits = (p.jobs + p.per_cta - 1) / p.per_cta;
+  const int runs = (int)std::min<int64_t>(p.jobs, std::max<int64_t>(1, (want + 2 * plan->n_tiles - 1) / (2 * plan->n_tiles)));
+  p.per_cta = (p.jobs + runs - 1) / runs;
+  p.runs = (p.jobs + p.per_cta - 1) / p.per_cta;
+  p.units = 2 * p.runs + (u_v ? 0 : 1);
   const int smem = 2 * palu::rb::stage_bytes(u_v ? std::max(r_k, r_v) : r_k) + palu::rb::kOutBytes;
   if (cudaFuncSetAttribute(palu::rb::palu_rebuild_kv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return cuda_check("cudaFuncSetAttribute(rebuild)");
-  palu::rb::palu_rebuild_kv_kernel<<<dim3(plan->n_tiles, splits), palu::rb::kThreads, smem, stream>>>(p);
+  palu::rb::palu_rebuild_kv_kernel<<<(unsigned)((int64_t)plan->n_tiles * p.units), palu::rb::kThreads, smem, stream>>>(p);
   return cuda_check("rebuild kernel launch");
 }
 
