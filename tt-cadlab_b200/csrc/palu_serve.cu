@@ -433,10 +433,22 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.per_cta = (p.jobs + runs - 1) / runs;
   p.runs = (p.jobs + p.per_cta - 1) / p.per_cta;
   p.units = 2 * p.runs + (u_v ? 0 : 1);
-  const int smem = 2 * palu::rb::stage_bytes(u_v ? std::max(r_k, r_v) : r_k) + palu::rb::kOutBytes;
-  if (cudaFuncSetAttribute(palu::rb::palu_rebuild_kv_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  const int smem = palu::rb::kStages * palu::rb::stage_bytes(u_v ? std::max(r_k, r_v) : r_k);
+  auto kern = palu::rb::palu_rebuild_kv_kernel<0>;
+  if (!u_v) switch (r_k) {
+      case 16: kern = palu::rb::palu_rebuild_kv_kernel<16>; break;
+      case 32: kern = palu::rb::palu_rebuild_kv_kernel<32>; break;
+      case 48: kern = palu::rb::palu_rebuild_kv_kernel<48>; break;
+      case 64: kern = palu::rb::palu_rebuild_kv_kernel<64>; break;
+      case 80: kern = palu::rb::palu_rebuild_kv_kernel<80>; break;
+      case 96: kern = palu::rb::palu_rebuild_kv_kernel<96>; break;
+      case 112: kern = palu::rb::palu_rebuild_kv_kernel<112>; break;
+      case 128: kern = palu::rb::palu_rebuild_kv_kernel<128>; break;
+      default: break;
+    }
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return cuda_check("cudaFuncSetAttribute(rebuild)");
-  palu::rb::palu_rebuild_kv_kernel<<<(unsigned)((int64_t)plan->n_tiles * p.units), palu::rb::kThreads, smem, stream>>>(p);
+  kern<<<(unsigned)((int64_t)plan->n_tiles * p.units), palu::rb::kThreads, smem, stream>>>(p);
   return cuda_check("rebuild kernel launch");
 }
 
