@@ -29,6 +29,8 @@
 // bounded; on expiry the CTA records a status code, all roles stop, copies and MMAs in flight are drained, TMEM is
 // freed and the rows not yet written get NaN.
 #pragma once
+#include <type_traits>
+
 #include "decode_tc.cuh"
 
 namespace palu {
@@ -40,7 +42,11 @@ constexpr int kPfThreads = 384;
 constexpr int kRows = 128;      // rows of a chain
 constexpr int kKeys = 128;      // keys of a tile
 constexpr int kQBytes = 2 * kBox, kKBytes = 2 * kBox;
-constexpr float kRescale = 8.f; // log2 of how far a row's maximum may outgrow its reference
+constexpr float kRescale = 16.f;  // log2 of how far a row's maximum may outgrow its reference
+#ifndef POLYE
+#define POLYE 4
+#endif
+constexpr int kPolyEvery = POLYE;  // every so manieth pair of exponentials is a polynomial
 
 // One work piece: key tiles [t0, t1) of one (query tile, KV head).
 struct PfPiece {
@@ -137,6 +143,24 @@ PALU_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// 2^x for x <= kRescale or so, two at a time, without the special-function unit: x = n + f with n the nearest integer
+// (added to 1.5 * 2^23, whose low bits then hold n), 2^f on [-1/2, 1/2] by the cubic with the least relative error (found
+// by Remez's exchange; 7.5e-5, a 50th of the rounding of P to bf16), n added to the exponent. Below 2^-126: about 2^-126.
+PALU_DEVINL uint64_t exp2_poly2(uint64_t x) {
+  float a, b;
+  unpack2(x, a, b);
+  const uint64_t y = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(y, pack2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), y);
+  uint64_t q = fma2(f, pack2(0.05517166852951050f, 0.05517166852951050f), pack2(0.24261112511157990f, 0.24261112511157990f));
+  q = fma2(q, f, pack2(0.69326096773147583f, 0.69326096773147583f));
+  q = fma2(q, f, pack2(0.99992805719375610f, 0.99992805719375610f));
+  float ta, tb;
+  unpack2(t, ta, tb);
+  unpack2(q, a, b);
+  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
+               __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
+}
 PALU_DEVINL void touch16(uint32_t* r) {  // a use of r that stays behind the volatile wait before it
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                     "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
@@ -164,6 +188,12 @@ PALU_DEVINL void tmem_st32p(uint32_t taddr, const uint32_t* r) {
 // Nonzero when one of the two bf16 in w is an infinity or a NaN (exponent all ones).
 PALU_DEVINL uint32_t nonfinite_bf16x2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
+PALU_DEVINL bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
+  return ok != 0;
+}
+
 template <bool ALIAS>
 __global__ void __launch_bounds__(kPfThreads, 1)
     palu_prefill_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -174,7 +204,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int w0 = p.cta_start[blockIdx.x], w1 = p.cta_start[blockIdx.x + 1];
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::OFF_MISC);
@@ -250,7 +280,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   const uint32_t tmem = *s_tmem;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 152;\n");
     if (warp == 8 && lane == 0) {
       // ============================== TMA producer ==============================
       tma_prefetch_map(&tm_q);
@@ -314,79 +344,98 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
         }
       }
-    } else if (warp == 9 && lane == 0) {
+    } else if (warp == 9) {
       // ============================== MMA issuer ==============================
-      // For each tile, chain 0 then chain 1: PV_c of the tile, then the chain's next S (the next piece's first one
-      // included), so that the chains' turns at the tensor cores alternate.
+      // The whole warp runs this and one elected lane issues, so that what the instructions take stays warp-uniform. For
+      // each tile, chain 0 then chain 1: PV_c of the tile, then the chain's next S (the next piece's first one included),
+      // so that the chains' turns at the tensor cores alternate.
       const uint32_t ID_QK = idesc_f16(kKeys, 1, false, false), ID_PV = idesc_f16(p.dv, 1, false, true);
-      int ns[2] = {0, 0}, np[2] = {0, 0}, nq[2] = {0, 0}, no[2] = {0, 0};  // S, PV, Q loads and pieces per chain so far
-      int kb = 0;                  // ring index of the piece's first tile
-      int ahead[2] = {-1, -1};     // the piece whose first S the chain has issued already
+      const uint64_t q_desc = sdesc(sbase + Lay::OFF_Q, 16, 1024), k_desc = sdesc(sbase + Lay::OFF_K, 16, 1024),
+                     v_desc = sdesc(sbase + Lay::OFF_V, kBox, 1024);
+      int ns0 = 0, ns1 = 0, np0 = 0, np1 = 0, nq0 = 0, nq1 = 0, no0 = 0, no1 = 0;  // S, PV, Q loads and pieces per chain so far
+      int kb = 0;                    // ring index of the piece's first tile
+      int ahead0 = -1, ahead1 = -1;  // the piece whose first S the chain has issued already
       bool ok = true;
-      auto issue_s = [&](int c, int n, bool first, bool last) -> bool {  // n: ring index of the K tile
-        if (first && !wait(bar(B_QF + c), nq[c]++ & 1)) return false;
-        if (!ALIAS && ns[c] >= 1 && !wait(bar(B_SR + c), (ns[c] - 1) & 1)) return false;
-        if (!wait(bar(B_KF + n % NS_K), (n / NS_K) & 1)) return false;
+      auto commit = [&](uint32_t b) {
+        if (elect_one()) mma_commit(b);
+        __syncwarp();
+      };
+      auto issue_s = [&](int c, int& ns, int& nq, int n, bool first, bool last) -> bool {  // n: ring index of the K tile
+        if (first && !wait_all(bar(B_QF + c), nq++ & 1)) return false;
+        if (!ALIAS && ns >= 1 && !wait_all(bar(B_SR + c), (ns - 1) & 1)) return false;
+        const int st = n % NS_K;
+        if (!wait_all(bar(B_KF + st), (n / NS_K) & 1)) return false;
         fence_after();
-        const uint32_t sK = sbase + Lay::OFF_K + (n % NS_K) * kKBytes, sQ = sbase + Lay::OFF_Q + c * kQBytes;
+        const uint64_t qd = q_desc + c * (kQBytes >> 4), kd = k_desc + st * (kKBytes >> 4);
+        const uint32_t d = tmem + Lay::S + 128 * c;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          mma_ss(tmem + Lay::S + 128 * c, sdesc(sQ + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024),
-                 sdesc(sK + (kk >> 2) * kBox + (kk & 3) * 32, 16, 1024), ID_QK, kk > 0);
-        mma_commit(bar(B_SF + c));
-        mma_commit(bar(B_KE + n % NS_K));
-        if (last) mma_commit(bar(B_QE + c));
-        ++ns[c];
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+            mma_ss(d, qd + off, kd + off, ID_QK, kk > 0);
+          }
+          mma_commit(bar(B_SF + c));
+          mma_commit(bar(B_KE + st));
+          if (last) mma_commit(bar(B_QE + c));
+        }
+        __syncwarp();
+        ++ns;
         return true;
       };
       for (int i = w0; ok && i < w1; ++i) {
         const PfPiece w = p.pieces[i];
         const PfChains ch = chains_of(w, p.ppt);
-        PfChains nx;
-        nx.n[0] = nx.n[1] = nx.nt = 0;
-        if (i + 1 < w1) nx = chains_of(p.pieces[i + 1], p.ppt);
-        for (int c = 0; ok && c < 2; ++c) {
-          if (ch.n[c] > 0) {
-            if (ahead[c] != i) ok = issue_s(c, kb, true, ch.n[c] == 1);
-          } else if (ch.nt > 0) {
-            mma_commit(bar(B_KE + kb % NS_K));
-          }
+        int nx0 = 0, nx1 = 0;
+        if (i + 1 < w1) {
+          const PfChains nx = chains_of(p.pieces[i + 1], p.ppt);
+          nx0 = nx.n[0];
+          nx1 = nx.n[1];
         }
+        auto begin = [&](int c, int n, int ahead, int& ns, int& nq) {
+          if (n > 0) {
+            if (ahead != i) ok = issue_s(c, ns, nq, kb, true, n == 1);
+          } else if (ch.nt > 0) {
+            commit(bar(B_KE + kb % NS_K));
+          }
+        };
+        begin(0, ch.n[0], ahead0, ns0, nq0);
+        if (ok) begin(1, ch.n[1], ahead1, ns1, nq1);
         for (int j = 0; ok && j < ch.nt; ++j) {
           const int n = kb + j, sv = n % NS_V;
-          if (!(ok = wait(bar(B_VF + sv), (n / NS_V) & 1))) break;
-          const uint32_t sV = sbase + Lay::OFF_V + sv * Lay::V_BYTES;
-          for (int c = 0; ok && c < 2; ++c) {
-            if (j >= ch.n[c]) {  // this chain sees nothing of the tile
-              mma_commit(bar(B_VE + sv));
-              if (j + 1 < ch.nt) mma_commit(bar(B_KE + (n + 1) % NS_K));
-              continue;
+          if (!(ok = wait_all(bar(B_VF + sv), (n / NS_V) & 1))) break;
+          const uint64_t vd = v_desc + sv * (Lay::V_BYTES >> 4);
+          auto step = [&](int c, int mine, int next, int& ns, int& np, int& nq, int& no, int& ahead) -> bool {
+            if (j >= mine) {  // this chain sees nothing of the tile
+              commit(bar(B_VE + sv));
+              if (j + 1 < ch.nt) commit(bar(B_KE + (n + 1) % NS_K));
+              return true;
             }
-            if (!(ok = wait(bar(B_PF + c), np[c] & 1))) break;
-            if (j == 0 && no[c] >= 1 && !(ok = wait(bar(B_OE + c), (no[c] - 1) & 1))) break;
+            if (!wait_all(bar(B_PF + c), np & 1)) return false;
+            if (j == 0 && no >= 1 && !wait_all(bar(B_OE + c), (no - 1) & 1)) return false;
             fence_after();
+            const uint32_t d = tmem + Lay::O + Lay::O_STEP * c, a = tmem + Lay::P + Lay::P_STEP * c;
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              mma_ts(tmem + Lay::O + Lay::O_STEP * c, tmem + Lay::P + Lay::P_STEP * c + 8 * kk,
-                     sdesc(sV + kk * 2048, kBox, 1024), ID_PV, (j | kk) != 0);
-            mma_commit(bar(B_OD + c));
-            mma_commit(bar(B_VE + sv));
-            ++np[c];
-            if (j + 1 < ch.n[c]) {
-              ok = issue_s(c, n + 1, false, j + 2 == ch.n[c]);
-            } else {
-              ++no[c];
-              if (j + 1 < ch.nt) mma_commit(bar(B_KE + (n + 1) % NS_K));
-              if (nx.n[c] > 0) {
-                ok = issue_s(c, kb + ch.nt, true, nx.n[c] == 1);
-                ahead[c] = i + 1;
-              }
+              for (int kk = 0; kk < 8; ++kk) mma_ts(d, a + 8 * kk, vd + kk * (2048 >> 4), ID_PV, (j | kk) != 0);
+              mma_commit(bar(B_OD + c));
+              mma_commit(bar(B_VE + sv));
             }
-          }
+            __syncwarp();
+            ++np;
+            if (j + 1 < mine) return issue_s(c, ns, nq, n + 1, false, j + 2 == mine);
+            ++no;
+            if (j + 1 < ch.nt) commit(bar(B_KE + (n + 1) % NS_K));
+            if (next > 0) {
+              ahead = i + 1;
+              return issue_s(c, ns, nq, kb + ch.nt, true, next == 1);
+            }
+            return true;
+          };
+          ok = step(0, ch.n[0], nx0, ns0, np0, nq0, no0, ahead0) && step(1, ch.n[1], nx1, ns1, np1, nq1, no1, ahead1);
         }
         kb += ch.nt;
       }
-      mma_commit(bar(B_DRAIN));
+      commit(bar(B_DRAIN));
       mbar_drain(bar(B_DRAIN), 0);
     } else if (warp >= 10) {
       // ============================== V of cut tiles ==============================
@@ -436,7 +485,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
     // ============================== softmax ==============================
     const int c = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -458,78 +507,114 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       for (int j = 0; j < nt; ++j, ++n_s) {
         if (!(ok = wait_all_inline(bar(B_SF + c), n_s & 1))) break;
         fence_after();
-        uint32_t s[128];
+        const int kb = (w.t0 + j) * kKeys;
+        const int nvis = kb + kKeys > ch.vis_first[c] ? vis - kb : kKeys;  // keys of the tile that this row sees
+        const bool cut = kb + kKeys > ch.vis_first[c];
+        uint32_t pk[64];
+        float top, m_new;  // the tile's maximum
+        uint64_t l2[2];
+        // P of the tile against m_ref, and the tile's maximum on the way: exponentials do not wait for it
+        auto stream = [&](auto is_cut) {
+          constexpr bool CUT = decltype(is_cut)::value;
+          const float mb = m_ref == -INFINITY ? 0.f : -m_ref * p.sl2;
+          const uint64_t sl2 = pack2(p.sl2, p.sl2), mb2 = pack2(mb, mb);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          l2[0] = l2[1] = 0;
+          uint32_t s[2][32];
+          tmem_ld32p(tS, s[0]);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld32p(tS + 32 * x, s + 32 * x);
-        tmem_wait_ld();
+          for (int q = 0; q < 4; ++q) {
+            uint32_t* x = s[q & 1];
+            tmem_wait_ld();
+            touch16(x);
+            touch16(x + 16);
+            if (q < 3) tmem_ld32p(tS + 32 * (q + 1), s[(q + 1) & 1]);
+            if constexpr (CUT) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x) touch16(s + 16 * x);
+              for (int i = 0; i < 32; ++i)
+                if (32 * q + i >= nvis) x[i] = 0xFF800000u;  // -inf
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) mx[y] = max3_nan(mx[y], __uint_as_float(x[i + y]), __uint_as_float(x[i + 4 + y]));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t y = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sl2, mb2);
+              uint64_t e;
+              if (!CUT && (i & (kPolyEvery - 1)) == kPolyEvery - 1) {  // masked keys are exactly 0
+                e = exp2_poly2(y);
+              } else {
+                float a, b;
+                unpack2(y, a, b);
+                e = pack2(fast_exp2(a), fast_exp2(b));
+              }
+              l2[i & 1] = add2(l2[i & 1], e);
+              float a, b;
+              unpack2(e, a, b);
+              pk[16 * q + i] = pack_bf16(a, b);
+            }
+          }
+          top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        };
+        if (j == 0) {  // a first reference: the tile's maximum
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            uint32_t x[32];
+            tmem_ld32p(tS + 32 * q, x);
+            tmem_wait_ld();
+            touch16(x);
+            touch16(x + 16);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * q + i >= nvis) x[i] = 0xFF800000u;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) mx[y] = max3_nan(mx[y], __uint_as_float(x[i + y]), __uint_as_float(x[i + 4 + y]));
+          }
+          m_ref = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        }
+        for (;;) {
+          if (cut) stream(std::true_type{});
+          else stream(std::false_type{});
+          m_new = max3_nan(m_true, top, top);
+          // A row whose maximum outgrew its reference by 2^kRescale or more takes it as the new reference (-inf - -inf is
+          // NaN: false); O and l follow, and the tile is done over.
+          const float use = m_ref == -INFINITY ? 0.f : m_ref;
+          const bool grow = (m_new - use) * p.sl2 > kRescale;
+          if (!__any_sync(0xffffffffu, grow)) break;
+          const float ref = grow ? m_new : m_ref;
+          const float alpha = m_ref == -INFINITY ? 0.f : (grow ? fast_exp2((m_ref - ref) * p.sl2) : 1.f);
+          if (j > 0) {
+            if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
+            fence_after();
+            for (int x = 0; x < p.dv; x += 16) {
+              uint32_t o[16];
+              tmem_ld16(tO + x, o);
+              tmem_wait_ld();
+              touch16(o);
+#pragma unroll
+              for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
+              tmem_st16(tO + x, o);
+            }
+            tmem_wait_st();
+          }
+          l *= alpha;
+          m_ref = ref;
+        }
+        if (!ok) break;
+        // PV of the tile before has read P (and every phase of the barrier is seen, so that its parity says which)
+        if (j > 0 && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
+        m_true = m_new;
         if (!ALIAS) {
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(B_SR + c));
         }
-        const int kb = (w.t0 + j) * kKeys;
-        if (kb + kKeys > ch.vis_first[c]) {
-          const int nvis = vis - kb;  // keys of the tile that this row sees
-#pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x >= nvis) s[x] = 0xFF800000u;  // -inf
-        }
-        float mx[4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) mx[a] = a == 0 ? m_true : __uint_as_float(s[a]);
-        mx[0] = max3_nan(mx[0], __uint_as_float(s[0]), __uint_as_float(s[4]));
-#pragma unroll
-        for (int a = 1; a < 4; ++a) mx[a] = max3_nan(mx[a], __uint_as_float(s[4 + a]), __uint_as_float(s[4 + a]));
-#pragma unroll
-        for (int x = 8; x < 128; x += 8)
-#pragma unroll
-          for (int a = 0; a < 4; ++a) mx[a] = max3_nan(mx[a], __uint_as_float(s[x + a]), __uint_as_float(s[x + 4 + a]));
-        m_true = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-        // the reference moves when it has to: at once from "none", and when outgrown by 2^8 or more
-        const bool grow = (m_true - m_ref) * p.sl2 > kRescale;  // -inf - -inf is NaN: false
-        if (j == 0) {
-          if (grow) m_ref = m_true;
-        } else if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? m_true : m_ref;
-          const float alpha = m_ref == -INFINITY ? 0.f : (grow ? fast_exp2((m_ref - m_new) * p.sl2) : 1.f);
-          if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
-          fence_after();
-          for (int x = 0; x < p.dv; x += 16) {
-            uint32_t o[16];
-            tmem_ld16(tO + x, o);
-            tmem_wait_ld();
-            touch16(o);
-#pragma unroll
-            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * alpha);
-            tmem_st16(tO + x, o);
-          }
-          tmem_wait_st();
-          l *= alpha;
-          m_ref = m_new;
-        }
-        const float mb = m_ref == -INFINITY ? 0.f : -m_ref * p.sl2;
-        const uint64_t sl2 = pack2(p.sl2, p.sl2), mb2 = pack2(mb, mb);
-        uint64_t l2[2] = {pack2(l, 0.f), pack2(0.f, 0.f)};
-        // PV of the tile before has read P (and every phase of the barrier is seen, so that its parity says which)
-        if (j > 0 && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const uint64_t y =
-                fma2(pack2(__uint_as_float(s[64 * h + 2 * x]), __uint_as_float(s[64 * h + 2 * x + 1])), sl2, mb2);
-            float a, b;
-            unpack2(y, a, b);
-            a = fast_exp2(a);
-            b = fast_exp2(b);
-            l2[x & 1] = add2(l2[x & 1], pack2(a, b));
-            pk[x] = pack_bf16(a, b);
-          }
-          tmem_st32p(tP + 32 * h, pk);
-        }
+        tmem_st32p(tP, pk);
+        tmem_st32p(tP + 32, pk + 32);
         tmem_wait_st();
         fence_before();
         __syncwarp();
@@ -537,7 +622,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         l2[0] = add2(l2[0], l2[1]);
         float la, lb;
         unpack2(l2[0], la, lb);
-        l = la + lb;
+        l += la + lb;
       }
       if (!ok) break;
       // ---- epilogue ----
@@ -545,8 +630,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
         fence_after();
       }
-      // a NaN or +infinity among the row's scores makes the row NaN
-      const bool lost = isnan(m_true) || m_true == INFINITY;
+      // a NaN or +infinity among the row's scores makes the row NaN, as do scores that are all -infinity
+      const bool lost = isnan(m_true) || m_true == INFINITY || (m_true == -INFINITY && vis > 0 && w.slot < 0);
       const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
       const size_t tok = (size_t)w.q0 + lpos;
       const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : (vis <= 0 ? 0.f : 1.f / l));
