@@ -42,11 +42,7 @@ constexpr int kPfThreads = 384;
 constexpr int kRows = 128;      // rows of a chain
 constexpr int kKeys = 128;      // keys of a tile
 constexpr int kQBytes = 2 * kBox, kKBytes = 2 * kBox;
-constexpr float kRescale = 16.f;  // log2 of how far a row's maximum may outgrow its reference
-#ifndef POLYE
-#define POLYE 4
-#endif
-constexpr int kPolyEvery = POLYE;  // every so manieth pair of exponentials is a polynomial
+constexpr float kOutgrown = 65536.f;  // a tile's sum of exponentials above which a row's reference is looked at
 
 // One work piece: key tiles [t0, t1) of one (query tile, KV head).
 struct PfPiece {
@@ -142,24 +138,6 @@ PALU_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-// 2^x for x <= kRescale or so, two at a time, without the special-function unit: x = n + f with n the nearest integer
-// (added to 1.5 * 2^23, whose low bits then hold n), 2^f on [-1/2, 1/2] by the cubic with the least relative error (found
-// by Remez's exchange; 7.5e-5, a 50th of the rounding of P to bf16), n added to the exponent. Below 2^-126: about 2^-126.
-PALU_DEVINL uint64_t exp2_poly2(uint64_t x) {
-  float a, b;
-  unpack2(x, a, b);
-  const uint64_t y = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t t = add2(y, pack2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), y);
-  uint64_t q = fma2(f, pack2(0.05517166852951050f, 0.05517166852951050f), pack2(0.24261112511157990f, 0.24261112511157990f));
-  q = fma2(q, f, pack2(0.69326096773147583f, 0.69326096773147583f));
-  q = fma2(q, f, pack2(0.99992805719375610f, 0.99992805719375610f));
-  float ta, tb;
-  unpack2(t, ta, tb);
-  unpack2(q, a, b);
-  return pack2(__uint_as_float(__float_as_uint(a) + (__float_as_uint(ta) << 23)),
-               __uint_as_float(__float_as_uint(b) + (__float_as_uint(tb) << 23)));
 }
 PALU_DEVINL void touch16(uint32_t* r) {  // a use of r that stays behind the volatile wait before it
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
@@ -402,7 +380,6 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         if (ok) begin(1, ch.n[1], ahead1, ns1, nq1);
         for (int j = 0; ok && j < ch.nt; ++j) {
           const int n = kb + j, sv = n % NS_V;
-          if (!(ok = wait_all(bar(B_VF + sv), (n / NS_V) & 1))) break;
           const uint64_t vd = v_desc + sv * (Lay::V_BYTES >> 4);
           auto step = [&](int c, int mine, int next, int& ns, int& np, int& nq, int& no, int& ahead) -> bool {
             if (j >= mine) {  // this chain sees nothing of the tile
@@ -410,26 +387,31 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               if (j + 1 < ch.nt) commit(bar(B_KE + (n + 1) % NS_K));
               return true;
             }
-            if (!wait_all(bar(B_PF + c), np & 1)) return false;
+            // the chain's next S: behind PV where P lies over S, else as soon as this S has been read
+            auto next_s = [&]() -> bool {
+              if (j + 1 < mine) return issue_s(c, ns, nq, n + 1, false, j + 2 == mine);
+              if (j + 1 < ch.nt) commit(bar(B_KE + (n + 1) % NS_K));
+              if (next > 0) {
+                ahead = i + 1;
+                return issue_s(c, ns, nq, kb + ch.nt, true, next == 1);
+              }
+              return true;
+            };
+            if (!ALIAS && !next_s()) return false;
+            if (!wait_all(bar(B_VF + sv), (n / NS_V) & 1) || !wait_all(bar(B_PF + c), np & 1)) return false;
             if (j == 0 && no >= 1 && !wait_all(bar(B_OE + c), (no - 1) & 1)) return false;
             fence_after();
             const uint32_t d = tmem + Lay::O + Lay::O_STEP * c, a = tmem + Lay::P + Lay::P_STEP * c;
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < 8; ++kk) mma_ts(d, a + 8 * kk, vd + kk * (2048 >> 4), ID_PV, (j | kk) != 0);
-              mma_commit(bar(B_OD + c));
+              if (!ALIAS || j + 1 == mine) mma_commit(bar(B_OD + c));
               mma_commit(bar(B_VE + sv));
             }
             __syncwarp();
             ++np;
-            if (j + 1 < mine) return issue_s(c, ns, nq, n + 1, false, j + 2 == mine);
-            ++no;
-            if (j + 1 < ch.nt) commit(bar(B_KE + (n + 1) % NS_K));
-            if (next > 0) {
-              ahead = i + 1;
-              return issue_s(c, ns, nq, kb + ch.nt, true, next == 1);
-            }
-            return true;
+            no += j + 1 == mine;
+            return !ALIAS || next_s();
           };
           ok = step(0, ch.n[0], nx0, ns0, np0, nq0, no0, ahead0) && step(1, ch.n[1], nx1, ns1, np1, nq1, no1, ahead1);
         }
@@ -491,7 +473,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tS = tlane + Lay::S + 128 * c, tP = tlane + Lay::P + Lay::P_STEP * c, tO = tlane + Lay::O + Lay::O_STEP * c;
     const int pos = row / p.rep, head = row - pos * p.rep;
-    int n_s = 0;  // tiles of this chain so far
+    int n_s = 0, n_o = 0;  // tiles and pieces with tiles of this chain so far
     bool ok = true;
     int i = w0;
     for (; i < w1; ++i) {
@@ -511,15 +493,13 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         const int nvis = kb + kKeys > ch.vis_first[c] ? vis - kb : kKeys;  // keys of the tile that this row sees
         const bool cut = kb + kKeys > ch.vis_first[c];
         uint32_t pk[64];
-        float top, m_new;  // the tile's maximum
-        uint64_t l2[2];
-        // P of the tile against m_ref, and the tile's maximum on the way: exponentials do not wait for it
+        float lt;  // the tile's sum
+        // P of the tile against m_ref, and its sum
         auto stream = [&](auto is_cut) {
           constexpr bool CUT = decltype(is_cut)::value;
           const float mb = m_ref == -INFINITY ? 0.f : -m_ref * p.sl2;
           const uint64_t sl2 = pack2(p.sl2, p.sl2), mb2 = pack2(mb, mb);
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          l2[0] = l2[1] = 0;
+          uint64_t l2[2] = {0, 0};
           uint32_t s[2][32];
           tmem_ld32p(tS, s[0]);
 #pragma unroll
@@ -535,29 +515,21 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                 if (32 * q + i >= nvis) x[i] = 0xFF800000u;  // -inf
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-#pragma unroll
-              for (int y = 0; y < 4; ++y) mx[y] = max3_nan(mx[y], __uint_as_float(x[i + y]), __uint_as_float(x[i + 4 + y]));
-#pragma unroll
             for (int i = 0; i < 16; ++i) {
               const uint64_t y = fma2(pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sl2, mb2);
-              uint64_t e;
-              if (!CUT && (i & (kPolyEvery - 1)) == kPolyEvery - 1) {  // masked keys are exactly 0
-                e = exp2_poly2(y);
-              } else {
-                float a, b;
-                unpack2(y, a, b);
-                e = pack2(fast_exp2(a), fast_exp2(b));
-              }
-              l2[i & 1] = add2(l2[i & 1], e);
               float a, b;
-              unpack2(e, a, b);
+              unpack2(y, a, b);
+              a = fast_exp2(a);
+              b = fast_exp2(b);
+              l2[i & 1] = add2(l2[i & 1], pack2(a, b));
               pk[16 * q + i] = pack_bf16(a, b);
             }
           }
-          top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+          float la, lb;
+          unpack2(add2(l2[0], l2[1]), la, lb);
+          lt = la + lb;
         };
-        if (j == 0) {  // a first reference: the tile's maximum
+        auto tile_max = [&]() -> float {
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
           for (int q = 0; q < 4; ++q) {
@@ -574,21 +546,30 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 #pragma unroll
               for (int y = 0; y < 4; ++y) mx[y] = max3_nan(mx[y], __uint_as_float(x[i + y]), __uint_as_float(x[i + 4 + y]));
           }
-          m_ref = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          return max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        };
+        if (j == 0) {  // a first reference: the tile's maximum
+          m_true = tile_max();
+          m_ref = isnan(m_true) ? 0.f : m_true;
         }
         for (;;) {
           if (cut) stream(std::true_type{});
           else stream(std::false_type{});
-          m_new = max3_nan(m_true, top, top);
-          // A row whose maximum outgrew its reference by 2^kRescale or more takes it as the new reference (-inf - -inf is
-          // NaN: false); O and l follow, and the tile is done over.
-          const float use = m_ref == -INFINITY ? 0.f : m_ref;
-          const bool grow = (m_new - use) * p.sl2 > kRescale;
-          if (!__any_sync(0xffffffffu, grow)) break;
-          const float ref = grow ? m_new : m_ref;
-          const float alpha = m_ref == -INFINITY ? 0.f : (grow ? fast_exp2((m_ref - ref) * p.sl2) : 1.f);
+          // The maximum is looked at where the sum says that it may have outgrown the reference (a sum of at most 2^16 holds no
+          // term above it; a NaN or infinity among the scores makes the sum NaN or huge), and while a row has no reference.
+          const bool look = have && (!(lt <= kOutgrown) || (m_ref == -INFINITY && nvis > 0));
+          if (!__any_sync(0xffffffffu, look)) break;
+          const float tm = tile_max();
+          float ref = m_ref;
+          if (look) {
+            m_true = max3_nan(m_true, tm, tm);
+            if (tm > m_ref && tm < INFINITY) ref = tm;
+          }
+          if (!__any_sync(0xffffffffu, ref != m_ref)) break;
+          // new references: O and l follow, and the tile is done over
+          const float alpha = ref == m_ref ? 1.f : (m_ref == -INFINITY ? 0.f : fast_exp2((m_ref - ref) * p.sl2));
           if (j > 0) {
-            if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
+            if (!ALIAS && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
             fence_after();
             for (int x = 0; x < p.dv; x += 16) {
               uint32_t o[16];
@@ -605,9 +586,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           m_ref = ref;
         }
         if (!ok) break;
-        // PV of the tile before has read P (and every phase of the barrier is seen, so that its parity says which)
-        if (j > 0 && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
-        m_true = m_new;
+        // PV of the tile before has read P; with P over S, S of this tile came behind it
+        if (!ALIAS && j > 0 && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
         if (!ALIAS) {
           fence_before();
           __syncwarp();
@@ -619,19 +599,17 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_PF + c));
-        l2[0] = add2(l2[0], l2[1]);
-        float la, lb;
-        unpack2(l2[0], la, lb);
-        l += la + lb;
+        l += lt;
       }
       if (!ok) break;
       // ---- epilogue ----
       if (nt > 0) {
-        if (!(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;
+        if (!(ok = wait_all_inline(bar(B_OD + c), (ALIAS ? n_o : n_s - 1) & 1))) break;
+        ++n_o;
         fence_after();
       }
       // a NaN or +infinity among the row's scores makes the row NaN, as do scores that are all -infinity
-      const bool lost = isnan(m_true) || m_true == INFINITY || (m_true == -INFINITY && vis > 0 && w.slot < 0);
+      const bool lost = isnan(m_true) || m_true == INFINITY || (m_ref == -INFINITY && vis > 0 && w.slot < 0);
       const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
       const size_t tok = (size_t)w.q0 + lpos;
       const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : (vis <= 0 ? 0.f : 1.f / l));
