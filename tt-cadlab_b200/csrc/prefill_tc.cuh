@@ -166,6 +166,11 @@ PALU_DEVINL void tmem_st32p(uint32_t taddr, const uint32_t* r) {
 // Nonzero when one of the two bf16 in w is an infinity or a NaN (exponent all ones).
 PALU_DEVINL uint32_t nonfinite_bf16x2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
+// w with its infinities and NaNs as zeros.
+PALU_DEVINL uint32_t finite_bf16x2(uint32_t w) {
+  const uint32_t f = nonfinite_bf16x2(w);
+  return w & ~((f >> 15 & 1u) * 0xFFFFu | (f >> 31) * 0xFFFF0000u);
+}
 PALU_DEVINL bool elect_one() {
   uint32_t ok;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
@@ -436,25 +441,26 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           const int r0 = max(0, w.vis0 - t * kKeys);         // rows below: every row of the item sees them
           const int r1 = min(kKeys, ch.vis_max - t * kKeys);  // rows from here on: none does
           uint32_t bad = 0;
-          for (int e = half * 32 + lane; e < (kKeys - r0) * chunks; e += 64) {
-            const int r = r0 + e / chunks, k = e % chunks;
-            uint4* at = reinterpret_cast<uint4*>(sV + (k >> 3) * kBox + r * 128 + (((k & 7) ^ (r & 7)) << 4));
+          for (int r = r0 + half * 32 + lane; r < kKeys; r += 64) {  // a row a lane
+            unsigned char* at = sV + r * 128;
             if (r >= r1) {
-              *at = make_uint4(0, 0, 0, 0);
+#pragma unroll 4
+              for (int k = 0; k < chunks; ++k) *reinterpret_cast<uint4*>(at + (k >> 3) * kBox + (((k & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
               continue;
             }
-            uint4 x = *at;
-            uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
-            uint32_t any = 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t f = nonfinite_bf16x2(xw[q]);
-              any |= f;
-              if (f & 0x8000u) xw[q] &= 0xFFFF0000u;
-              if (f & 0x80000000u) xw[q] &= 0x0000FFFFu;
+#pragma unroll 4
+            for (int k = 0; k < chunks; ++k) {
+              uint4* x = reinterpret_cast<uint4*>(at + (k >> 3) * kBox + (((k & 7) ^ (r & 7)) << 4));
+              uint4 v = *x;
+              if (nonfinite_bf16x2(v.x) | nonfinite_bf16x2(v.y) | nonfinite_bf16x2(v.z) | nonfinite_bf16x2(v.w)) {
+                bad = 1;
+                v.x = finite_bf16x2(v.x);
+                v.y = finite_bf16x2(v.y);
+                v.z = finite_bf16x2(v.z);
+                v.w = finite_bf16x2(v.w);
+                *x = v;
+              }
             }
-            if (any) *at = x;
-            bad |= any;
           }
           if (bad) s_bad[i & 3] = i + 1;
           fence_proxy_async();  // these reads and writes before the tensor core's reads and the slot's next copy
@@ -476,8 +482,11 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     int n_s = 0, n_o = 0;  // tiles and pieces with tiles of this chain so far
     bool ok = true;
     int i = w0;
+    PfPiece ahead;  // the next piece, read while this one is worked on
+    if (w0 < w1) ahead = p.pieces[w0];
     for (; i < w1; ++i) {
-      const PfPiece w = p.pieces[i];
+      const PfPiece w = ahead;
+      if (i + 1 < w1) ahead = p.pieces[i + 1];
       const PfChains ch = chains_of(w, p.ppt);
       if (!ch.active[c]) continue;
       const int lpos = c * p.ppt + pos;                       // position within the item
@@ -529,10 +538,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           unpack2(add2(l2[0], l2[1]), la, lb);
           lt = la + lb;
         };
-        auto tile_max = [&]() -> float {
+        auto tile_max = [&](int chunks) -> float {
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < chunks; ++q) {
             uint32_t x[32];
             tmem_ld32p(tS + 32 * q, x);
             tmem_wait_ld();
@@ -548,8 +557,8 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           }
           return max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]);
         };
-        if (j == 0) {  // a first reference: the tile's maximum
-          m_true = tile_max();
+        if (j == 0) {  // a first reference: the maximum of the first keys
+          m_true = tile_max(1);
           m_ref = isnan(m_true) ? 0.f : m_true;
         }
         for (;;) {
@@ -559,7 +568,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
           // term above it; a NaN or infinity among the scores makes the sum NaN or huge), and while a row has no reference.
           const bool look = have && (!(lt <= kOutgrown) || (m_ref == -INFINITY && nvis > 0));
           if (!__any_sync(0xffffffffu, look)) break;
-          const float tm = tile_max();
+          const float tm = tile_max(4);
           float ref = m_ref;
           if (look) {
             m_true = max3_nan(m_true, tm, tm);
@@ -612,29 +621,35 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const bool lost = isnan(m_true) || m_true == INFINITY || (m_ref == -INFINITY && vis > 0 && w.slot < 0);
       const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
       const size_t tok = (size_t)w.q0 + lpos;
-      const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : (vis <= 0 ? 0.f : 1.f / l));
+      const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : 1.f / l);
       float* po = p.ws_o + ((size_t)w.slot * 2 * kRows + c * kRows + row) * p.dv;  // used with a slot only
       __nv_bfloat16* go = p.out + (tok * p.n_q + w.kvh * p.rep + head) * p.dv;
-      for (int x = 0; x < p.dv; x += 16) {
-        uint32_t o[16];
+      for (int x = 0; x < p.dv; x += 32) {  // the last 16 columns may be behind d_v: read and dropped
+        uint32_t o[32];
         if (nt > 0) {
-          tmem_ld16(tO + x, o);
+          tmem_ld32p(tO + x, o);
           tmem_wait_ld();
           touch16(o);
+          touch16(o + 16);
+          if (x + 32 >= p.dv) {  // O has been read: the next piece's first PV may overwrite it
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_OE + c));
+          }
         } else {
 #pragma unroll
-          for (int y = 0; y < 16; ++y) o[y] = 0;
+          for (int y = 0; y < 32; ++y) o[y] = 0;
         }
         if (!have) continue;
         if (bad) {  // non-finite values of the partly visible V rows, to the rows that see them
-          const int k_lo = max(w.vis0, w.t0 * kKeys), k_hi = min(vis, w.t1 * kKeys);
-          for (int k = max(k_lo, 0); k < k_hi; ++k) {
+          const int k_lo = max(max(w.vis0, w.t0 * kKeys), 0), k_hi = min(vis, w.t1 * kKeys), nx = min(32, p.dv - x);
+          for (int k = k_lo; k < k_hi; ++k) {
             const __nv_bfloat16* vr = p.v + (int64_t)(w.k0 + k) * p.v_tok + w.kvh * p.v_head + x;
-            for (int y = 0; y < 16; ++y) {
+            for (int y = 0; y < nx; ++y) {
               const float f = __bfloat162float(vr[y]);
               if (!(fabsf(f) < INFINITY)) {
 #pragma unroll
-                for (int z = 0; z < 16; ++z)
+                for (int z = 0; z < 32; ++z)
                   if (z == y) o[z] = __float_as_uint(__uint_as_float(o[z]) + f);
               }
             }
@@ -642,26 +657,22 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         }
         if (w.slot >= 0) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-            reinterpret_cast<uint4*>(po + x)[y] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
-        } else {
-          uint32_t h[8];
-#pragma unroll
           for (int y = 0; y < 8; ++y)
+            if (x + 4 * y < p.dv) reinterpret_cast<uint4*>(po + x)[y] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
+        } else {
+          uint32_t h[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y)
             h[y] = vis <= 0 ? 0u : pack_bf16(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
-          reinterpret_cast<uint4*>(go + x)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-          reinterpret_cast<uint4*>(go + x)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (x + 8 * y < p.dv) reinterpret_cast<uint4*>(go + x)[y] = make_uint4(h[4 * y], h[4 * y + 1], h[4 * y + 2], h[4 * y + 3]);
         }
       }
       if (w.slot >= 0 && have) {
         float* ml = p.ws_ml + ((size_t)w.slot * 2 * kRows + c * kRows + row) * 2;
         ml[0] = lost ? NAN : (m_ref == -INFINITY ? -INFINITY : m_ref * p.sl2);
         ml[1] = l;
-      }
-      if (nt > 0) {
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_OE + c));
       }
     }
     if (!ok) {  // the rows that this chain still owed become NaN
