@@ -1,6 +1,7 @@
 // C ABI of the operators around the decode step: the plan and attention of packed prompts. Validation, planning and
 // dispatch on the host; the kernels live in the .cuh files next to it.
 #include <algorithm>
+#include <atomic>
 #include <new>
 #include <vector>
 
@@ -14,6 +15,18 @@
 using namespace palu::abi;
 
 namespace {
+
+// cudaFuncSetAttribute's dynamic shared memory limit, set once per kernel and device (`done`: one word per kernel, a bit per
+// device; racing threads set the same value). Kernels whose size varies are given the largest they can need.
+int allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return cuda_check(what);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return PALU_OK;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return cuda_check(what);
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return PALU_OK;
+}
 
 // ---- the plan of a packed batch -----------------------------------------------------------------------
 
@@ -368,8 +381,8 @@ int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* 
     constexpr bool A = decltype(alias)::value;
     auto kern = palu::pf::palu_prefill_tc_kernel<A>;
     const int smem = palu::pf::PfLayout<A>::TOTAL;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return cuda_check("cudaFuncSetAttribute(prefill)");
+    static std::atomic<uint64_t> done{0};
+    if (int st = allow_smem((const void*)kern, smem, done, "cudaFuncSetAttribute(prefill)")) return st;
     kern<<<plan->n_ctas, palu::pf::kPfThreads, smem, stream>>>(mq, mk, mv, p);
     return cuda_check("prefill kernel launch");
   };
@@ -473,8 +486,8 @@ int palu_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t r
   while (c < 8 && rows * c * 2 * 3 <= 13 * device_sms() && vocab >= palu::lp::kThreads * 16 * c * 2) c *= 2;
   const int smem = palu::lp::kStages * palu::lp::kStageBytes;
   auto kern = dtype == PALU_F32 ? palu::lp::palu_token_logprobs_kernel<float> : palu::lp::palu_token_logprobs_kernel<__nv_bfloat16>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return cuda_check("cudaFuncSetAttribute(logprobs)");
+  static std::atomic<uint64_t> done[2];
+  if (int st = allow_smem((const void*)kern, smem, done[dtype == PALU_F32], "cudaFuncSetAttribute(logprobs)")) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, slots / c)) * c));
   cfg.blockDim = dim3(palu::lp::kThreads);

@@ -41,7 +41,7 @@ using namespace palu::tc;
 constexpr int kPfThreads = 384;
 constexpr int kRows = 128;      // rows of a chain
 constexpr int kKeys = 128;      // keys of a tile
-constexpr int kQBytes = 2 * kBox, kKBytes = 2 * kBox;
+constexpr int kQBytes = 2 * kBox, kKBytes = 2 * kBox, kOutBytes = 32 * 128;
 constexpr float kOutgrown = 65536.f;  // a tile's sum of exponentials above which a row's reference is looked at
 
 // One work piece: key tiles [t0, t1) of one (query tile, KV head).
@@ -63,7 +63,7 @@ struct PfParams {
   const PfPiece* pieces;
   const int32_t* cta_start;  // [gridDim.x + 1]
   __nv_bfloat16* out;        // [T][n_q][d_v]
-  float* ws_o;               // [slots][256][d_v]
+  float* ws_o;               // [slots][2][d_v][128]: a chain's rows innermost
   float* ws_ml;              // [slots][256][2]
   int* status;
   const __nv_bfloat16* v;    // [Tk][n_kv][d_v] with the strides below (elements)
@@ -76,13 +76,18 @@ struct PfParams {
 
 template <bool ALIAS>
 struct PfLayout {
-  static constexpr int NS_K = 3, NS_V = ALIAS ? 2 : 3;
+  static constexpr int NS_K = 2, NS_V = ALIAS ? 2 : 3;
+  // Registers a thread of the role warps and of the softmax warps: 4 x 32 and 8 x 32 threads of the 384 x 168 launched. (us for
+  // 8192 tokens with 152 / 176, 136 / 184, 120 / 192: d_v 128 470, 485, 506; d_v 64 442, 429, 443.)
+  static constexpr int ROLE_REGS = ALIAS ? 152 : 136, SOFT_REGS = ALIAS ? 176 : 184;
+  static_assert(4 * 32 * ROLE_REGS + 8 * 32 * SOFT_REGS <= kPfThreads * 168, "the warpgroups' shares of the launch's registers");
   static constexpr int V_BYTES = ALIAS ? 2 * kBox : kBox;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * kQBytes;
   static constexpr int OFF_V = OFF_K + NS_K * kKBytes;
-  static constexpr int OFF_MISC = OFF_V + NS_V * V_BYTES;
-  static constexpr int TOTAL = OFF_MISC + 512 + 1024;
+  static constexpr int OFF_OUT = OFF_V + NS_V * V_BYTES;  // 32 rows x 64 results (bf16) a softmax warp
+  static constexpr int OFF_MISC = OFF_OUT + 8 * kOutBytes;
+  static constexpr int TOTAL = OFF_MISC + 512 + kRows * 4 + 1024;
   // TMEM columns
   static constexpr uint32_t S = 0;                       // + 128 c
   static constexpr uint32_t P = ALIAS ? 0 : 256;         // + P_STEP c
@@ -201,6 +206,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
                 B_DRAIN = B_OE + 2, B_COUNT = B_DRAIN + 1;
   static_assert(B_COUNT * 8 + 64 <= 512, "misc area");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  int* s_row = reinterpret_cast<int*>(smem + Lay::OFF_MISC + 512);  // [128] a row's position << 8 | query head
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_bad = reinterpret_cast<volatile int*>(s_tmem + 2);  // [4]: 1 + index of the last piece with non-finite V
 
@@ -251,6 +257,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
+  if (threadIdx.x < kRows) s_row[threadIdx.x] = (threadIdx.x / p.rep) << 8 | (threadIdx.x % p.rep);
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
                  "r"(kTmemCols)
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   const uint32_t tmem = *s_tmem;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 152;\n");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(Lay::ROLE_REGS));
     if (warp == 8 && lane == 0) {
       // ============================== TMA producer ==============================
       tma_prefetch_map(&tm_q);
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     }
     __syncwarp();
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(Lay::SOFT_REGS));
     // ============================== softmax ==============================
     const int c = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -620,53 +627,70 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       // a NaN or +infinity among the row's scores makes the row NaN, as do scores that are all -infinity
       const bool lost = isnan(m_true) || m_true == INFINITY || (m_ref == -INFINITY && vis > 0 && w.slot < 0);
       const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
-      const size_t tok = (size_t)w.q0 + lpos;
-      const float inv = w.slot >= 0 ? 1.f : (lost ? NAN : 1.f / l);
-      float* po = p.ws_o + ((size_t)w.slot * 2 * kRows + c * kRows + row) * p.dv;  // used with a slot only
-      __nv_bfloat16* go = p.out + (tok * p.n_q + w.kvh * p.rep + head) * p.dv;
-      for (int x = 0; x < p.dv; x += 32) {  // the last 16 columns may be behind d_v: read and dropped
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_ld32p(tO + x, o);
-          tmem_wait_ld();
-          touch16(o);
-          touch16(o + 16);
-          if (x + 32 >= p.dv) {  // O has been read: the next piece's first PV may overwrite it
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_OE + c));
+      const float inv = lost ? NAN : 1.f / l;
+      for (int x = 0; x < p.dv; x += 64) {
+        unsigned char* stage = smem + Lay::OFF_OUT + warp * kOutBytes;
+        const int width = min(64, p.dv - x);
+#pragma unroll 1
+        for (int y = 0; y < width; y += 32) {  // the last 16 columns may be behind d_v: read and dropped
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_ld32p(tO + x + y, o);
+            tmem_wait_ld();
+            touch16(o);
+            touch16(o + 16);
+            if (x + y + 32 >= p.dv) {  // O has been read: the next piece's first PV may overwrite it
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(B_OE + c));
+            }
+          } else {
+#pragma unroll
+            for (int z = 0; z < 32; ++z) o[z] = 0;
           }
-        } else {
+          if (bad && have) {  // non-finite values of the partly visible V rows, to the rows that see them
+            const int k_lo = max(max(w.vis0, w.t0 * kKeys), 0), k_hi = min(vis, w.t1 * kKeys), n = min(32, width - y);
+            for (int k = k_lo; k < k_hi; ++k) {
+              const __nv_bfloat16* vr = p.v + (int64_t)(w.k0 + k) * p.v_tok + w.kvh * p.v_head + x + y;
+              for (int z = 0; z < n; ++z) {
+                const float f = __bfloat162float(vr[z]);
+                if (!(fabsf(f) < INFINITY)) {
 #pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = 0;
-        }
-        if (!have) continue;
-        if (bad) {  // non-finite values of the partly visible V rows, to the rows that see them
-          const int k_lo = max(max(w.vis0, w.t0 * kKeys), 0), k_hi = min(vis, w.t1 * kKeys), nx = min(32, p.dv - x);
-          for (int k = k_lo; k < k_hi; ++k) {
-            const __nv_bfloat16* vr = p.v + (int64_t)(w.k0 + k) * p.v_tok + w.kvh * p.v_head + x;
-            for (int y = 0; y < nx; ++y) {
-              const float f = __bfloat162float(vr[y]);
-              if (!(fabsf(f) < INFINITY)) {
-#pragma unroll
-                for (int z = 0; z < 32; ++z)
-                  if (z == y) o[z] = __float_as_uint(__uint_as_float(o[z]) + f);
+                  for (int q = 0; q < 32; ++q)
+                    if (q == z) o[q] = __float_as_uint(__uint_as_float(o[q]) + f);
+                }
               }
             }
           }
+          if (w.slot >= 0) {
+            float* po = p.ws_o + (((size_t)w.slot * 2 + c) * p.dv + x + y) * kRows + row;
+#pragma unroll
+            for (int z = 0; z < 32; ++z)
+              if (y + z < width) po[z * kRows] = __uint_as_float(o[z]);
+          } else {
+            // through shared memory, so that 8 lanes write 128 bytes of a row: chunk k of row r at chunk k ^ r & 7 (straight from
+            // the registers, every store touched 32 lines: 3000 to 4000 cycles a piece at d_v 128)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              uint32_t h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                h[q] = vis <= 0 ? 0u : pack_bf16(__uint_as_float(o[8 * z + 2 * q]) * inv, __uint_as_float(o[8 * z + 2 * q + 1]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((y >> 3) + z) ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          }
         }
-        if (w.slot >= 0) {
+        if (w.slot < 0) {
+          __syncwarp();
+          const int k = lane & 7;
 #pragma unroll
-          for (int y = 0; y < 8; ++y)
-            if (x + 4 * y < p.dv) reinterpret_cast<uint4*>(po + x)[y] = make_uint4(o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]);
-        } else {
-          uint32_t h[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y)
-            h[y] = vis <= 0 ? 0u : pack_bf16(__uint_as_float(o[2 * y]) * inv, __uint_as_float(o[2 * y + 1]) * inv);
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (x + 8 * y < p.dv) reinterpret_cast<uint4*>(go + x)[y] = make_uint4(h[4 * y], h[4 * y + 1], h[4 * y + 2], h[4 * y + 3]);
+          for (int z = 0; z < 8; ++z) {
+            const int r = 4 * z + (lane >> 3), at = s_row[(warp & 3) * 32 + r], lp = c * p.ppt + (at >> 8);
+            if ((at >> 8) < p.ppt && lp < w.npos && 8 * k < width)
+              *reinterpret_cast<uint4*>(p.out + (((size_t)w.q0 + lp) * p.n_q + w.kvh * p.rep + (at & 255)) * p.dv + x + 8 * k) =
+                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
+          }
+          __syncwarp();
         }
       }
       if (w.slot >= 0 && have) {
@@ -698,44 +722,47 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   }
 }
 
-// Joins the records of the items that were cut along the keys: one warp per row, with w_s = 2^(m_s - max m),
-// o = sum_s w_s O_s / sum_s w_s l_s. Bound by reading the records (fp32).
+// Joins the records of the items that were cut along the keys: with w_s = 2^(m_s - max m),
+// o = sum_s w_s O_s / sum_s w_s l_s. A block joins 32 rows (a lane a row, a warp every eighth column) and writes them
+// through shared memory. Bound by reading the records (fp32).
 __global__ void __launch_bounds__(256) palu_prefill_merge_kernel(const PfMerge* merges, const PfParams p) {
+  __shared__ float s_o[32][129];
   const PfMerge w = merges[blockIdx.x];
-  const int lane = threadIdx.x & 31;
-  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < 2 * kRows; r += gridDim.y * 8) {
-    const int c = r >> 7, row = r & 127, pos = row / p.rep, head = row - pos * p.rep, lpos = c * p.ppt + pos;
-    if (pos >= p.ppt || lpos >= w.npos) continue;
-    const bool empty = w.vis0 + lpos <= 0;
-    float m = -INFINITY;
-    bool lost = false;
-    for (int s = 0; s < w.n; ++s) {
-      const float ms = p.ws_ml[((size_t)(w.slot0 + s) * 2 * kRows + r) * 2];
-      lost |= isnan(ms);
-      m = fmaxf(m, ms);
-    }
-    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    const int x = lane * 4;
-    for (int s = 0; s < w.n; ++s) {
-      const size_t rec = (size_t)(w.slot0 + s) * 2 * kRows + r;
-      const float ms = p.ws_ml[rec * 2];
-      if (ms == -INFINITY) continue;  // the row saw nothing of this piece
-      const float wt = fast_exp2(ms - m);
-      l += wt * p.ws_ml[rec * 2 + 1];
-      if (x < p.dv) {
-        const float4 v = *reinterpret_cast<const float4*>(p.ws_o + rec * p.dv + x);
-        o[0] += wt * v.x;
-        o[1] += wt * v.y;
-        o[2] += wt * v.z;
-        o[3] += wt * v.w;
-      }
-    }
-    if (x < p.dv) {
-      const float inv = lost ? NAN : 1.f / l;
-      uint2 h = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-      if (empty) h = make_uint2(0u, 0u);
-      *reinterpret_cast<uint2*>(p.out + (((size_t)w.q0 + lpos) * p.n_q + w.kvh * p.rep + head) * p.dv + x) = h;
-    }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.y * 32 + lane, c = r >> 7, row = r & 127, lpos = c * p.ppt + row / p.rep;
+  if (c * p.ppt + (blockIdx.y * 32 & 127) / p.rep >= w.npos) return;  // the block's first row is behind the item
+  const bool have = row / p.rep < p.ppt && lpos < w.npos, empty = w.vis0 + lpos <= 0;
+  float m = -INFINITY;
+  bool lost = false;
+  for (int s = 0; s < w.n; ++s) {
+    const float ms = have ? p.ws_ml[((size_t)(w.slot0 + s) * 2 * kRows + r) * 2] : -INFINITY;
+    lost |= isnan(ms);
+    m = fmaxf(m, ms);
+  }
+  float l = 0.f, o[16];
+#pragma unroll
+  for (int y = 0; y < 16; ++y) o[y] = 0.f;
+  for (int s = 0; s < w.n; ++s) {
+    const size_t rec = (size_t)(w.slot0 + s) * 2 * kRows + r;
+    const float ms = have ? p.ws_ml[rec * 2] : -INFINITY;
+    if (ms == -INFINITY) continue;  // the row saw nothing of this piece
+    const float wt = fast_exp2(ms - m);
+    l += wt * p.ws_ml[rec * 2 + 1];
+    const float* po = p.ws_o + (((size_t)(w.slot0 + s) * 2 + c) * p.dv) * kRows + row;
+#pragma unroll
+    for (int y = 0; y < 16; ++y)
+      if (warp + 8 * y < p.dv) o[y] += wt * po[(warp + 8 * y) * kRows];
+  }
+  const float inv = lost ? NAN : 1.f / l;
+#pragma unroll
+  for (int y = 0; y < 16; ++y)
+    if (warp + 8 * y < p.dv) s_o[lane][warp + 8 * y] = empty ? 0.f : o[y] * inv;
+  __syncthreads();
+  for (int e = threadIdx.x; e < 32 * (p.dv / 2); e += 256) {
+    const int rr = e / (p.dv / 2), x = e - rr * (p.dv / 2), row2 = (blockIdx.y * 32 + rr) & 127, pos = row2 / p.rep, lp = c * p.ppt + pos;
+    if (pos >= p.ppt || lp >= w.npos) continue;
+    *reinterpret_cast<uint32_t*>(p.out + (((size_t)w.q0 + lp) * p.n_q + w.kvh * p.rep + row2 % p.rep) * p.dv + 2 * x) =
+        pack_bf16(s_o[rr][2 * x], s_o[rr][2 * x + 1]);
   }
 }
 

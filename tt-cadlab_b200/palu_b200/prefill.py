@@ -16,6 +16,7 @@ import torch
 from palu_b200 import _lib
 
 HEAD_DIM = 128
+_SCALE = HEAD_DIM ** -0.5
 
 
 def _lengths(x, what: str):
@@ -75,7 +76,7 @@ class PrefillPlan:
         stream = torch.cuda.current_stream(self.device)
         stream.synchronize()
         self._stream = stream.cuda_stream
-        self.info_ptr = ctypes.byref(self.info)
+        self.info_ptr, self.data_ptr = ctypes.byref(self.info), self.data.data_ptr()
 
     def workspace_bytes(self, d_v: int) -> int:
         n = self._ws_bytes.get(d_v)
@@ -97,15 +98,16 @@ class PrefillPlan:
 def _heads(t: torch.Tensor, what: str, tokens: int, heads: int, width: Optional[int], device) -> torch.Tensor:
     """A bf16 [tokens, heads, width] tensor on the plan's device, its last dimension contiguous and its rows 16-byte
     aligned (copied where they are not)."""
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[1] != heads or (width is not None and t.shape[2] != width):
-        raise RuntimeError(f"{what} must be [{tokens}, {heads}, {width if width is not None else 'd_v'}], got {tuple(t.shape)}")
-    if t.device != device:
-        raise RuntimeError(f"{what} is on {t.device}, the plan on {device}")
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or (width is not None and shape[2] != width):
+        raise RuntimeError(f"{what} must be [{tokens}, {heads}, {width if width is not None else 'd_v'}], got {tuple(shape)}")
     if t.dtype != torch.bfloat16:
         raise RuntimeError(f"{what} must be bf16, got {t.dtype}")
-    s = t.stride()
-    if s[2] != 1 or s[1] % 8 or s[0] % 8 or s[0] <= 0 or s[1] <= 0 or t.data_ptr() % 16:
-        t = t.contiguous() if not t.is_contiguous() or t.data_ptr() % 16 == 0 else t.clone()
+    if t.device != device:
+        raise RuntimeError(f"{what} is on {t.device}, the plan on {device}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or s1 % 8 or s0 % 8 or s0 <= 0 or s1 <= 0 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -117,27 +119,29 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Prefil
     Query i of a sequence sees its keys 0 .. i + k_len - q_len; one that sees none gives 0. What lies behind a query's
     last key does not reach its result, whatever it holds. q, k and v may be strided (slices of a fused projection);
     the products accumulate in fp32, the probabilities are rounded to bf16 for the second one."""
-    _lib.require_cuda(q, k, v, out)
-    q = _heads(q, "q", plan.q_tokens, plan.n_q_heads, HEAD_DIM, plan.device)
-    k = _heads(k, "k", plan.k_tokens, plan.n_kv_heads, HEAD_DIM, plan.device)
-    v = _heads(v, "v", plan.k_tokens, plan.n_kv_heads, None, plan.device)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        _lib.require_cuda(q, k, v, out)
+    dev = plan.device
+    q = _heads(q, "q", plan.q_tokens, plan.n_q_heads, HEAD_DIM, dev)
+    k = _heads(k, "k", plan.k_tokens, plan.n_kv_heads, HEAD_DIM, dev)
+    v = _heads(v, "v", plan.k_tokens, plan.n_kv_heads, None, dev)
     d_v = v.shape[2]
-    shape = (plan.q_tokens, plan.n_q_heads, d_v)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-    elif tuple(out.shape) != shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != q.device:
-        raise RuntimeError(f"out must be a contiguous bf16 {shape} tensor on {q.device}")
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+        out = torch.empty(plan.q_tokens, plan.n_q_heads, d_v, dtype=torch.bfloat16, device=dev)
+    elif (tuple(out.shape) != (plan.q_tokens, plan.n_q_heads, d_v) or out.dtype != torch.bfloat16 or not out.is_contiguous()
+          or out.device != dev):
+        raise RuntimeError(f"out must be a contiguous bf16 {(plan.q_tokens, plan.n_q_heads, d_v)} tensor on {dev}")
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
             return prefill_attn(q, k, v, plan, scale=scale, out=out)
     need = plan.workspace_bytes(d_v)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    stream = _lib.stream_handle(q.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    stream = _lib.stream_handle(dev)
     plan.use_on(stream)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
     _lib.check(_lib.load().palu_prefill_attn(
-        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-        v.stride(1), out.data_ptr(), d_v, plan.info_ptr, plan.data.data_ptr(), _lib.ptr(ws), need,
-        HEAD_DIM ** -0.5 if scale is None else float(scale), stream))
+        q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), d_v, plan.info_ptr,
+        plan.data_ptr, None if ws is None else ws.data_ptr(), need, _SCALE if scale is None else float(scale), stream))
     return out
 
 
@@ -192,5 +196,5 @@ def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor
     plan.use_on(stream)
     _lib.check(_lib.load().palu_rebuild_kv(
         k_latent.data_ptr(), v_latent.data_ptr(), u_k.data_ptr(), _lib.ptr(u_v), cos.data_ptr(), sin.data_ptr(), pg,
-        plan.info_ptr, plan.data.data_ptr(), k.data_ptr(), v.data_ptr(), n_groups, r_k, r_v, S, stream))
+        plan.info_ptr, plan.data_ptr, k.data_ptr(), v.data_ptr(), n_groups, r_k, r_v, S, stream))
     return k, v

@@ -31,28 +31,32 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     Equal logits are ordered by the lower id. A negative token stands for none and gives 0; one at or past the vocabulary
     gives NaN. A logit of -inf has probability 0; a row of -inf only, or with a NaN or +inf in it, has no distribution:
     its log probabilities and entropy are NaN. Everything is computed in fp32."""
-    _lib.require_cuda(logits, tokens)
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.shape[1] < 1:
-        raise RuntimeError(f"logits must be bf16 or fp32 [N, vocab], got {logits.dtype} {tuple(logits.shape)}")
+    dtype, dev = logits.dtype, logits.device
+    if not logits.is_cuda or not tokens.is_cuda:
+        _lib.require_cuda(logits, tokens)
+    if logits.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float32) or logits.shape[1] < 1:
+        raise RuntimeError(f"logits must be bf16 or fp32 [N, vocab], got {dtype} {tuple(logits.shape)}")
     n, vocab = logits.shape
-    if tuple(tokens.shape) != (n,) or tokens.dtype not in (torch.int64, torch.int32):
+    wide = tokens.dtype == torch.int64
+    if tokens.dim() != 1 or tokens.shape[0] != n or not (wide or tokens.dtype == torch.int32):
         raise RuntimeError(f"tokens must be [{n}] int64 or int32, got {tokens.dtype} {tuple(tokens.shape)}")
-    if tokens.device != logits.device:
-        raise RuntimeError(f"tokens are on {tokens.device}, logits on {logits.device}")
+    if tokens.device != dev:
+        raise RuntimeError(f"tokens are on {tokens.device}, logits on {dev}")
     top = int(top)
-    if not 0 <= top <= min(MAX_TOP, vocab):
+    if not 0 <= top <= MAX_TOP or top > vocab:
         raise RuntimeError(f"top must be in [0, {min(MAX_TOP, vocab)}] (at most 32, at most the vocabulary), got {top}")
-    if logits.device.index != torch.cuda.current_device():
-        with torch.cuda.device(logits.device):
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
             return token_logprobs(logits, tokens, top)
-    if logits.stride(1) != 1 or (n > 1 and logits.stride(0) < vocab):
+    ld, step = logits.stride()
+    if step != 1 or (n > 1 and ld < vocab):
         logits = logits.contiguous()
+        ld = vocab
     tokens = tokens.contiguous()
-    dev, f32 = logits.device, torch.float32
-    lp, ent = torch.empty(n, dtype=f32, device=dev), torch.empty(n, dtype=f32, device=dev)
-    tv, ti = torch.empty(n, top, dtype=f32, device=dev), torch.empty(n, top, dtype=torch.int64, device=dev)
+    empty, f32 = torch.empty, torch.float32
+    lp, ent, tv = empty(n, dtype=f32, device=dev), empty(n, dtype=f32, device=dev), empty(n, top, dtype=f32, device=dev)
+    ti = empty(n, top, dtype=torch.int64, device=dev)
     _lib.check(_lib.load().palu_token_logprobs(
-        logits.data_ptr(), logits.stride(0), _lib.PALU_F32 if logits.dtype == torch.float32 else _lib.PALU_BF16, n, vocab,
-        tokens.data_ptr(), int(tokens.dtype == torch.int64), top, lp.data_ptr(), ent.data_ptr(), tv.data_ptr(), ti.data_ptr(),
-        _lib.stream_handle(logits.device)))
+        logits.data_ptr(), ld, _lib.PALU_BF16 if dtype == torch.bfloat16 else _lib.PALU_F32, n, vocab, tokens.data_ptr(), wide, top,
+        lp.data_ptr(), ent.data_ptr(), tv.data_ptr(), ti.data_ptr(), _lib.stream_handle(dev)))
     return TokenLogprobs(lp, ent, tv, ti)
