@@ -13,6 +13,8 @@ Per decode step (attention.py:585-733):
 
 ``forward_prefill`` fills the caches for a prompt and returns the prompt's attention output with torch
 SDPA on the rebuilt K / V (the reference runs its prefill on full K / V too, attention.py:382-516).
+``forward_prefill_packed`` is its form for serving: prompts of different lengths without padding, or chunks
+of prompts behind their cached prefix, on the library's rebuild and packed attention (``prefill``).
 
 Paged caches: with ``paged_attention_config`` (tt_transformers' argument, which the reference accepts and
 asserts is None, attention.py:83-86) the caches are [max_num_blocks, n_groups, block_size, r] and the
@@ -30,7 +32,7 @@ from typing import Optional
 
 import torch
 
-from palu_b200 import fused
+from palu_b200 import fused, prefill
 from palu_b200.convert import LowRank, reverse_permute
 from palu_b200.shard import KVShard, all_reduce_layer_output, layer_output_partial
 
@@ -323,3 +325,43 @@ class PaluAttention:
         attn = attn.transpose(1, 2).reshape(B * P, self.nh, -1)
         y = self._out(attn).view(B, P, self.dim)
         return y.view(1, 1, P, self.dim) if shape4 else y
+
+    @torch.no_grad()
+    def forward_prefill_packed(self, x: torch.Tensor, plan: "prefill.PrefillPlan",
+                               page_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Prefill of a packed batch (``prefill.PrefillPlan`` with this rank's head counts): x [plan.q_tokens, dim], sequence s's
+        tokens at the positions k_lens[s] - q_lens[s] .. k_lens[s] - 1 of cache row plan.rows[s], whose earlier positions are
+        cached already (none for a whole prompt). Writes the tokens' latents into the caches, rebuilds each row's keys and
+        values from the cached (bf16) latents and returns the causal attention output [q_tokens, dim] fp32. q, K, V and the
+        probabilities are bf16 on this path (fp32 in ``forward_prefill``). bf16 caches, contiguous or paged (``page_table``: the
+        whole table, by cache row; tokens whose page it does not name are not written and read as zero latents)."""
+        if self.latent_dtype != "bf16" or self.k_cache.dtype != torch.bfloat16 or self.device.type != "cuda":
+            raise RuntimeError("packed prefill needs bf16 latent caches on a CUDA device")
+        if (plan.n_q_heads, plan.n_kv_heads) != (self.nh, self.nkv):
+            raise RuntimeError(f"the plan is for {plan.n_q_heads} / {plan.n_kv_heads} heads, the layer has {self.nh} / {self.nkv}")
+        if tuple(x.shape) != (plan.q_tokens, self.dim):
+            raise RuntimeError(f"x must be [{plan.q_tokens}, {self.dim}], got {tuple(x.shape)}")
+        if any(q > k for q, k in zip(plan.q_lens, plan.k_lens)) or max(plan.k_lens, default=0) > self.max_seq:
+            raise RuntimeError(f"a sequence's queries are among its keys, at most max_seq {self.max_seq} of them")
+        T = plan.q_tokens
+        pt = self._check_pages(page_table)
+        rows_held = self.max_batch if pt is None else pt.shape[0]
+        if max(plan.rows, default=0) >= rows_held or (T and len(set(plan.rows)) != len(plan.rows)):
+            raise RuntimeError(f"the plan's cache rows must be distinct and below {rows_held}")
+        if T == 0:
+            return torch.zeros(0, self.dim, device=self.device)
+        xb = x.to(self.device)
+        qkv = (xb if xb.dtype == self.proj_dtype else xb.float().to(self.proj_dtype)) @ self.w_qkv.T
+        rows, pos = plan.token_index()
+        nq, nk = self.nh * self.head_dim, self.ng * self.r_k
+        q = self._rotate(qkv[:, :nq].float().view(T, self.nh, self.head_dim), pos).to(torch.bfloat16)
+        k_new = qkv[:, nq:nq + nk].reshape(T, self.ng, self.r_k).to(torch.bfloat16)
+        v_new = qkv[:, nq + nk:].reshape(T, self.ng, self.r_v).to(torch.bfloat16)
+        if pt is None:
+            self.k_cache[rows, :, pos], self.v_cache[rows, :, pos] = k_new, v_new
+        else:  # each token as a row of its own whose only page is the one that holds its position
+            bs = self.paged.block_size
+            fused.append_latents(k_new, v_new, pos % bs, self.k_cache, self.v_cache, page_table=pt[rows, pos // bs][:, None])
+        k, v = prefill.rebuild_kv(self.k_cache, self.v_cache, self.u_k, self.cos, self.sin, plan,
+                                  u_v=None if self.u_v is None else self.u_v[0], page_table=pt)
+        return self._out(prefill.prefill_attn(q, k, v, plan, scale=self.scale))

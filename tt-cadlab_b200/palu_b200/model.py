@@ -22,8 +22,11 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from palu_b200 import fused
+from palu_b200 import scoring
 from palu_b200.attention import LLAMA3_SCALING, PagedAttentionConfig, PaluAttention
 from palu_b200.convert import LowRank
+from palu_b200.paging import PagePool
+from palu_b200.prefill import PrefillPlan
 from palu_b200.shard import KVShard
 
 
@@ -221,6 +224,75 @@ class PaluDecoder:
                                               page_table=page_table)
             h = h + self._mlp(L, rms_norm(h, L["ffn_norm"], self.cfg.norm_eps).reshape(B * P, -1)).view(B, P, -1)
         return self._logits(h[:, -1])
+
+    # ---- packed prompts, scoring, pages -----------------------------------------------------------------
+    def prefill_plan(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None,
+                     rows: Optional[Sequence[int]] = None) -> PrefillPlan:
+        """The layout of a packed batch for this rank's heads (``prefill.PrefillPlan``)."""
+        a = self.layers[0]["attn"]
+        return PrefillPlan(q_lens, k_lens, n_q_heads=a.nh, n_kv_heads=a.nkv, rows=rows, device=self.device)
+
+    @torch.no_grad()
+    def prefill_packed(self, tokens: torch.Tensor, plan: PrefillPlan, page_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Packed tokens [plan.q_tokens] through every layer (``PaluAttention.forward_prefill_packed``): fills the caches and
+        returns the final normed hidden states [q_tokens, dim] in the weights' dtype, for ``lm_head`` or ``score``."""
+        h = self.embed[tokens.to(self.device)].float()                                      # [T, dim]
+        if plan.q_tokens == 0:
+            return h.to(self.dtype)
+        norm = fused.add_rms_norm if self._fused_elementwise() else None
+        eps = self.cfg.norm_eps
+        if norm is None:
+            for L in self.layers:
+                h = h + L["attn"].forward_prefill_packed(rms_norm(h, L["attn_norm"], eps), plan, page_table)
+                h = h + self._mlp(L, rms_norm(h, L["ffn_norm"], eps))
+            return rms_norm(h, self.norm, eps).to(self.dtype)
+        x = norm(h, None, self.layers[0]["attn_norm"], eps)
+        for i, L in enumerate(self.layers):
+            x = norm(h, L["attn"].forward_prefill_packed(x, plan, page_table), L["ffn_norm"], eps)
+            nxt = self.layers[i + 1]["attn_norm"] if i + 1 < len(self.layers) else self.norm
+            x = norm(h, self._mlp(L, x, fp32=False), nxt, eps)
+        return x
+
+    @torch.no_grad()
+    def prefill_packed_logits(self, tokens: torch.Tensor, plan: PrefillPlan,
+                              page_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``prefill_logits`` for a packed batch: the logits [sequences, vocab] fp32 of each sequence's last token (sequences
+        without a token have no row)."""
+        x = self.prefill_packed(tokens, plan, page_table)
+        lens = [n for n in plan.q_lens if n]
+        last = (torch.tensor(lens).cumsum(0) - 1).to(self.device)
+        return (x[last] @ self.lm_head.t()).float()
+
+    @torch.no_grad()
+    def score(self, tokens: torch.Tensor, plan: PrefillPlan, page_table: Optional[torch.Tensor] = None, *, top: int = 0,
+              chunk: int = 4096) -> scoring.TokenLogprobs:
+        """Log probabilities of a packed batch's own tokens (what perplexity is made of), with the entropy and ``top``
+        alternatives at each: row t is for the token behind packed token t in its sequence; a sequence's last token has none
+        (log probability 0). The LM head runs on ``chunk`` tokens at a time."""
+        x = self.prefill_packed(tokens, plan, page_table)
+        nxt = torch.full((plan.q_tokens,), -1, dtype=torch.int64, device=self.device)
+        nxt[:-1] = tokens.to(self.device)[1:]
+        last = [i for i in torch.tensor([n for n in plan.q_lens if n]).cumsum(0).sub(1).tolist()]
+        nxt[last] = -1
+        parts = [scoring.token_logprobs(x[a:a + chunk] @ self.lm_head.t(), nxt[a:a + chunk], top)
+                 for a in range(0, max(plan.q_tokens, 1), chunk)]
+        return scoring.TokenLogprobs(*(torch.cat(t) for t in zip(*parts)))
+
+    @torch.no_grad()
+    def decode_logprobs(self, tokens: torch.Tensor, pos: torch.Tensor, page_table: Optional[torch.Tensor] = None, *, top: int = 0):
+        """One greedy decode step with what a server answers next to the token: next tokens [B] and their ``TokenLogprobs``."""
+        logits = self.decode_logits(tokens, pos, page_table)
+        nxt = logits.argmax(-1)
+        return nxt, scoring.token_logprobs(logits, nxt, top)
+
+    def page_pool(self, rows: int) -> PagePool:
+        """A ``PagePool`` over every layer's paged K and V caches with ``rows`` table rows; its ``table`` is the page table of
+        the prefill and decode calls."""
+        a = self.layers[0]["attn"]
+        if a.paged is None:
+            raise RuntimeError("a page pool needs paged caches (paged_attention_config)")
+        caches = [c for L in self.layers for c in (L["attn"].k_cache, L["attn"].v_cache)]
+        return PagePool(caches, rows=rows, blocks_per_row=-(-a.max_seq // a.paged.block_size))
 
     # ---- CUDA graph of one decode step ------------------------------------------------------------------
     def capture_decode(self, batch: int, page_table: Optional[torch.Tensor] = None) -> "DecodeGraph":

@@ -70,7 +70,7 @@ class PrefillPlan:
         _lib.check(st)
         self.q_tokens, self.k_tokens = int(self.info.q_tokens), int(self.info.k_tokens)
         self.n_q_heads, self.n_kv_heads = int(n_q_heads), int(n_kv_heads)
-        self._ws_bytes = {}
+        self._ws_bytes, self._index = {}, None
         self.host = host[:int(self.info.bytes)]
         self.data = self.host.to(self.device)
         stream = torch.cuda.current_stream(self.device)
@@ -87,7 +87,20 @@ class PrefillPlan:
     def use_on(self, stream: int) -> None:
         """Keep the plan's memory until work queued on ``stream`` is done, if that is not the stream it was made on."""
         if stream != self._stream and not torch.cuda.is_current_stream_capturing():
-            self.data.record_stream(torch.cuda.current_stream(self.device))
+            for t in (self.data, self._index):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream(self.device))
+
+    def token_index(self):
+        """Per packed query token its cache row and its position ([q_tokens] int64 each, on the device; laid out once): the
+        queries of a sequence stand at the last of its keys' positions."""
+        if self._index is None:
+            ql, kl = torch.tensor(self.q_lens), torch.tensor(self.k_lens)
+            start = torch.repeat_interleave(kl - ql - (ql.cumsum(0) - ql), ql)
+            host = torch.stack([torch.repeat_interleave(torch.tensor(self.rows), ql), torch.arange(self.q_tokens) + start])
+            self._index = host.to(self.device)
+            torch.cuda.current_stream(self.device).synchronize()
+        return self._index[0], self._index[1]
 
     def status(self) -> int:
         """Read and clear the plan's status word: nonzero when a bounded device wait of a call expired (the rows that it
