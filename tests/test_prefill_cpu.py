@@ -57,10 +57,10 @@ def test_every_query_tile_is_covered_once(q_lens, k_lens, n_q, n_kv):
         else:
             m = joined[key]
             assert sorted(x[2] for x in parts) == list(range(m[4], m[4] + m[5]))
-    # 64-token tiles of the cached rows, for the rebuild
+    # 128-token tiles of the cached rows, for the rebuild
     at = 0
     for t in tiles:
-        assert t[2] == at and 0 < t[3] <= 64
+        assert t[2] == at and 0 < t[3] <= 128
         at += t[3]
     assert at == sum(k_lens)
 
@@ -72,8 +72,8 @@ def test_long_keys_behind_few_queries_are_split():
 
 
 def test_cache_rows_reach_the_rebuild_tiles():
-    tiles = plan([0, 0], [70, 3], 4, 4, rows=[5, 2])[4]
-    assert tiles == [[5, 0, 0, 64], [5, 64, 64, 6], [2, 0, 70, 3]]
+    tiles = plan([0, 0], [140, 3], 4, 4, rows=[5, 2])[4]
+    assert tiles == [[5, 0, 0, 128], [5, 128, 128, 12], [2, 0, 140, 3]]
 
 
 @pytest.mark.parametrize("args,needle", [

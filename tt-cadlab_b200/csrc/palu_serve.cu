@@ -134,7 +134,8 @@ void make_lists(const int32_t* q_lens, const int32_t* k_lens, const int32_t* row
       const int n = std::min(step, ql - a), vis0 = kl - ql + a + 1, last = vis0 + n - 1;
       items.push_back({q0 + a, n, vis0, k0, last > 0 ? (last + palu::pf::kKeys - 1) / palu::pf::kKeys : 0});
     }
-    for (int a = 0; a < kl; a += 64) out.tiles.push_back(make_int4(rows ? rows[s] : s, a, k0 + a, std::min(64, kl - a)));
+    for (int a = 0; a < kl; a += palu::rb::kTokens)
+      out.tiles.push_back(make_int4(rows ? rows[s] : s, a, k0 + a, std::min(palu::rb::kTokens, kl - a)));
     q0 += ql;
     k0 += kl;
   }
@@ -439,30 +440,64 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.r_k = r_k;
   p.r_v = r_v;
   p.max_seq = max_seq;
+  p.status = reinterpret_cast<int*>(const_cast<void*>(plan_data));
+  p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
   p.jobs = u_v ? 2 * p.n_kv : p.n_kv;
-  // heads per CTA: as many as leave every SM a few CTAs (a CTA reads its tokens' table rows once)
-  const int64_t want = 8LL * device_sms();
-  const int runs = (int)std::min<int64_t>(p.jobs, std::max<int64_t>(1, (want + 2 * plan->n_tiles - 1) / (2 * plan->n_tiles)));
-  p.per_cta = (p.jobs + runs - 1) / runs;
-  p.runs = (p.jobs + p.per_cta - 1) / p.per_cta;
-  p.units = 2 * p.runs + (u_v ? 0 : 1);
-  const int smem = palu::rb::kStages * palu::rb::stage_bytes(u_v ? std::max(r_k, r_v) : r_k);
-  auto kern = palu::rb::palu_rebuild_kv_kernel<0>;
-  if (!u_v) switch (r_k) {
-      case 16: kern = palu::rb::palu_rebuild_kv_kernel<16>; break;
-      case 32: kern = palu::rb::palu_rebuild_kv_kernel<32>; break;
-      case 48: kern = palu::rb::palu_rebuild_kv_kernel<48>; break;
-      case 64: kern = palu::rb::palu_rebuild_kv_kernel<64>; break;
-      case 80: kern = palu::rb::palu_rebuild_kv_kernel<80>; break;
-      case 96: kern = palu::rb::palu_rebuild_kv_kernel<96>; break;
-      case 112: kern = palu::rb::palu_rebuild_kv_kernel<112>; break;
-      case 128: kern = palu::rb::palu_rebuild_kv_kernel<128>; break;
-      default: break;
-    }
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return cuda_check("cudaFuncSetAttribute(rebuild)");
-  kern<<<(unsigned)((int64_t)plan->n_tiles * p.units), palu::rb::kThreads, smem, stream>>>(p);
-  return cuda_check("rebuild kernel launch");
+  // runs of heads: as many as it takes to give every SM a unit (a unit reads its tokens' table rows once)
+  const int sms = device_sms();
+  const int runs = (int)std::min<int64_t>(p.jobs, std::max<int64_t>(1, (sms + plan->n_tiles - 1) / plan->n_tiles));
+  p.per_unit = (p.jobs + runs - 1) / runs;
+  p.runs = (p.jobs + p.per_unit - 1) / p.per_unit;
+  if ((int64_t)plan->n_tiles * p.runs > (1 << 30)) return fail(PALU_ERR_INVALID, "rebuild: too many tiles");
+  p.units = plan->n_tiles * p.runs;
+  const int r_max = u_v ? std::max(r_k, r_v) : r_k;
+  p.a_bytes = (r_max + 63) / 64 * palu::tc::kBox;
+  p.u_bytes = (r_max * 256 + 1023) / 1024 * 1024;
+  const int slot = p.a_bytes + p.u_bytes, outs = 8 * palu::rb::kOutBytes, room = palu::tc::kSmemBudget - palu::rb::kFixedSmem;
+  p.out_bufs = room - 2 * outs >= slot ? 2 : 1;
+  p.ring = std::min(palu::rb::kMaxRing, (room - p.out_bufs * outs) / slot);
+  const int smem = palu::rb::kFixedSmem + p.out_bufs * outs + p.ring * slot;
+  // tensor maps: latents by (row of the cache, latent head) or (page, latent head), U by rows of 128
+  CUtensorMap mk, mv, muk, muv, mko, mvo;
+  const int64_t items = pages ? (int64_t)pages->n_blocks * n_groups : (int64_t)(plan->max_row + 1) * n_groups;
+  const int64_t seq = pages ? pages->block_size : max_seq;
+  auto latents = [&](CUtensorMap* m, const void* base, int r, const char* what) -> int {
+    const cuuint64_t dims[3] = {(cuuint64_t)r, (cuuint64_t)seq, (cuuint64_t)items};
+    const cuuint64_t str[2] = {(cuuint64_t)r * 2, (cuuint64_t)seq * r * 2};
+    const cuuint32_t box[3] = {64, pages ? (cuuint32_t)pages->block_size : (cuuint32_t)palu::rb::kTokens, 1};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, str, box, what);
+  };
+  auto factors = [&](CUtensorMap* m, const void* base, int r, const char* what) -> int {
+    const cuuint64_t dims[2] = {128, (cuuint64_t)p.n_kv * r};
+    const cuuint64_t str[1] = {256};
+    const cuuint32_t box[2] = {64, (cuuint32_t)r};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, str, box, what);
+  };
+  if (int st = latents(&mk, k_lat, r_k, "k_lat")) return st;
+  if (int st = factors(&muk, u_k, r_k, "u_k")) return st;
+  auto results = [&](CUtensorMap* m, void* base, const char* what) -> int {
+    const cuuint64_t dims[3] = {128, (cuuint64_t)p.n_kv, (cuuint64_t)plan->k_tokens};
+    const cuuint64_t str[2] = {256, (cuuint64_t)p.n_kv * 256};
+    const cuuint32_t box[3] = {64, 1, 32};
+    return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, str, box, what);
+  };
+  if (int st = results(&mko, k_out, "k_out")) return st;
+  mv = mk;
+  muv = muk;
+  mvo = mko;
+  if (u_v) {
+    if (int st = results(&mvo, v_out, "v_out")) return st;
+    if (int st = latents(&mv, v_lat, r_v, "v_lat")) return st;
+    if (int st = factors(&muv, u_v, r_v, "u_v")) return st;
+  }
+  static std::atomic<uint64_t> done{0};
+  if (int st = allow_smem((const void*)palu::rb::palu_rebuild_kv_kernel, palu::tc::kSmemBudget, done, "cudaFuncSetAttribute(rebuild)")) return st;
+  palu::rb::palu_rebuild_kv_kernel<<<std::min(p.units, sms), palu::rb::kThreads, smem, stream>>>(mk, mv, muk, muv, mko, mvo, p);
+  if (int st = cuda_check("rebuild kernel launch")) return st;
+  if (u_v) return PALU_OK;
+  const int heads = (int)std::min<int64_t>(n_groups, std::max<int64_t>(1, 4LL * sms / plan->n_tiles));
+  palu::rb::palu_gather_latents_kernel<<<dim3(plan->n_tiles, heads), palu::rb::kGatherThreads, 0, stream>>>(p);
+  return cuda_check("gather kernel launch");
 }
 
 int palu_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int64_t rows, int32_t vocab, const void* tokens, int32_t tokens64,

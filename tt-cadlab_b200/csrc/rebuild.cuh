@@ -3,221 +3,384 @@
 // with R_pos rotating the pairs (2f, 2f + 1) by the table's cos and sin. Products accumulate in fp32, the rotation is
 // fp32, and each result is rounded to bf16 once (half a step, 2^-8).
 //
-// Bound by memory: at rank 64 a token and head reads 128 B and writes 256 B for 16 kFLOP, a sixth of what the tensor
-// cores could do meanwhile, so warp-level mma.sync reaches the same bound as tcgen05 would and keeps the accumulators in
-// registers, where a rotation pair sits in one thread and the rotation is free. What it takes is loads in flight: a CTA
-// takes 64 tokens and half of the head dims for all its heads (with all 128 dims, accumulators and table rows left room
-// for 8 warps an SM, and 32 rows of 8192 tokens took 610 us), copies latents and U (cp.async) two heads ahead of the products, keeps its tokens' table rows in registers for all heads, and writes whole 128-byte lines.
-// Gathered values are a copy by CTAs of their own. The CTAs of a tile are neighbours, so that its latents and table
-// rows come from DRAM once.
+// Bound by memory: at rank 64 a token and head reads 128 B and writes 256 B for 16 kFLOP. The products run on tcgen05, which
+// reads its operands from shared memory by itself: with warp-level mma.sync the fragments' trips through the load/store
+// pipe (144 wavefronts of 128 B per 16 x 64 results) were what bound, 316 us for 32 rows of 8192 tokens at rank 64.
+//
+// A unit is 128 tokens of a row and a run of heads; CTAs are persistent, one an SM. Per head: TMA brings the latents' tile
+// (once per latent head; from a paged cache one box a page) and U_h, tcgen05.mma writes D = c U (128 x 128, f32) to one of
+// four TMEM buffers, and 8 warps turn it into results: a thread has a token's row and 64 head dims (a warp reads the 32 TMEM
+// lanes of its quarter), with the token's 32 frequencies of the table in registers for all heads of the unit; the rows leave
+// through shared memory by TMA (stored by the lanes, the stores took half of the warps' time: 196 us for 32 x 8192 tokens). Two warps bring the next unit's table rows to shared memory meanwhile
+// (loaded by the warps that use them, between units, they cost as much as the unit's heads). Warps 0..7: results, 8: TMA
+// producer, 9: MMA issuer, 10 and 11: table. Every wait is
+// bounded; on expiry the plan's status word is set and the unit's remaining results become NaN.
 #pragma once
-#include "palu_common.cuh"
+#include "prefill_tc.cuh"
 
 namespace palu {
 namespace rb {
 
-constexpr int kTokens = 64, kThreads = 128;
+using namespace palu::tc;
+using palu::pf::elect_one;
+using palu::pf::touch16;
+using palu::pf::tmem_ld32p;
+
+constexpr int kTokens = 128, kThreads = 384, kDBufs = 4, kMaxRing = 4;
+constexpr int kRoleRegs = 104, kResultRegs = 200;  // of the 168 x 384 launched
+static_assert(4 * 32 * kRoleRegs + 8 * 32 * kResultRegs <= kThreads * 168, "the warpgroups' shares of the launch's registers");
+constexpr int kOutBytes = 32 * 128;          // a warp's 32 rows x 64 results
+constexpr int kTableBytes = kTokens * 512;  // a token's 64 cosines, then its 64 sines (fp32)
+constexpr int kFixedSmem = kTableBytes + 512 + 1024;  // and the rings, and one or two sets of the 8 warps' result buffers
 
 struct Params {
   const __nv_bfloat16 *k_lat, *v_lat, *u_k, *u_v;  // u_v null: V is gathered
   const float *cos, *sin;                          // [>= positions][128], each frequency twice
   __nv_bfloat16 *k_out, *v_out;
-  const int4* tiles;                               // row, first position, packed token, tokens (<= 64)
+  const int4* tiles;                               // row, first position, packed token, tokens (<= 128)
   const int32_t* page_table;                       // null: contiguous [B][n_groups][max_seq][r]
   int table_ld, blk_shift, n_blocks;
   int n_kv, n_groups, r_k, r_v, max_seq;
-  int jobs, per_cta, runs;                         // heads to multiply (K, then V), of a CTA, and runs of them
-  int units;                                       // CTAs of a tile: 2 halves of each run, then one for gathered values
+  int jobs, per_unit, runs, units;                 // heads to multiply (K, then V), per unit, runs of them, units in all
+  int ring, a_bytes, u_bytes, out_bufs;            // slots of the latent and the U ring, bytes of one; result buffers a warp
+  int* status;
+  unsigned long long wait_ns;
 };
 
-// Rows of a staged tile are padded by 16 bytes: 8 rows then start 4 banks apart (r / 2 + 4 or 36 words, odd multiples
-// of 4).
-__host__ __device__ constexpr int lat_stride(int r) { return r * 2 + 16; }
-constexpr int kHalf = 64, kUStride = kHalf * 2 + 16;
-constexpr int kStages = 3;
-// A warp's results go where its 16 latent rows were: their room is the larger of the two.
-__host__ __device__ constexpr int lat_bytes(int r) { return kTokens * (lat_stride(r) > kUStride ? lat_stride(r) : kUStride); }
-__host__ __device__ constexpr int stage_bytes(int r) { return lat_bytes(r) + r * kUStride; }
-
-// Row of a cached position in a cache of any width, for latent head 0 (each further head `step` rows on), or -1 where the
-// page table names no block.
-PALU_DEVINL int64_t cache_row(const Params& p, int row, int pos) {
-  if (!p.page_table) return (int64_t)row * p.n_groups * p.max_seq + pos;
-  const int b = p.page_table[(int64_t)row * p.table_ld + (pos >> p.blk_shift)];
-  if ((unsigned)b >= (unsigned)p.n_blocks) return -1;
-  return (((int64_t)b * p.n_groups) << p.blk_shift) + (pos & ((1 << p.blk_shift) - 1));
-}
-PALU_DEVINL void stsm_x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-               : "memory");
+PALU_DEVINL void cp_async4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
-// R: the K latents' width where it is at most 128 and values are not rebuilt, known to the compiler (the loops over it are
-// then straight code); 0: any widths, K and V heads.
-template <int R>
-__global__ void __launch_bounds__(kThreads, 4) palu_rebuild_kv_kernel(const Params p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  const int4 tile = p.tiles[blockIdx.x / p.units];
-  const int unit = blockIdx.x % p.units;
-  const int row = tile.x, pos0 = tile.y, count = tile.w;
-  const int64_t tok0 = tile.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  // 8 threads copy a token's row, 16 bytes each: token tid / 8 and every 16th after it
-  const int t8 = tid >> 3, c8 = tid & 7, step = p.page_table ? 1 << p.blk_shift : p.max_seq;
-  int64_t at[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) at[i] = t8 + 16 * i < count ? cache_row(p, row, pos0 + t8 + 16 * i) : -1;
-
-  if (unit == 2 * p.runs) {  // gathered V: the latent heads as they are
-    const int ch = p.r_v >> 3;
-    for (int g = 0; g < p.n_groups; ++g)
-      for (int c = c8; c < ch; c += 8) {
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (at[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(p.v_lat + (at[i] + (int64_t)g * step) * p.r_v + c * 8);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t8 + 16 * i < count)
-            *reinterpret_cast<uint4*>(p.v_out + ((tok0 + t8 + 16 * i) * p.n_groups + g) * p.r_v + c * 8) = v[i];
-      }
-    return;
-  }
-
-  const int half = unit & 1, j0 = (unit >> 1) * p.per_cta, j1 = min(p.jobs, j0 + p.per_cta);
-  const int stage_sz = stage_bytes(R ? R : (p.u_v ? max(p.r_k, p.r_v) : p.r_k));
-  const uint32_t sb = smem_u32(smem);
+// A head to multiply.
+struct Job {
+  bool is_v, new_a, last_of_a;  // new_a: its latents differ from the job's before it; last_of_a: from the one's behind it
+  int h, g, r;
+};
+PALU_DEVINL Job job_of(const Params& p, int job, int j0, int j1) {
   const int gs = p.n_kv / p.n_groups;
+  Job x;
+  x.is_v = job >= p.n_kv;
+  x.h = x.is_v ? job - p.n_kv : job;
+  x.g = x.h / gs;
+  x.r = x.is_v ? p.r_v : p.r_k;
+  x.new_a = job == j0 || x.h % gs == 0;
+  x.last_of_a = job == j1 - 1 || (x.h + 1) % gs == 0;
+  return x;
+}
 
-  // The next head to copy: its latents (4 token rows) and U, as pointers that move from head to head.
-  int h_l = 0, in_group = 0, r_l = 0;
-  bool v_l = false;
-  const __nv_bfloat16 *src_l[4], *u_l = nullptr;
-  auto seek = [&](int job) {
-    v_l = R == 0 && job >= p.n_kv;
-    h_l = v_l ? job - p.n_kv : job;
-    r_l = R ? R : (v_l ? p.r_v : p.r_k);
-    const int g = h_l / gs;
-    in_group = h_l - g * gs;
-    const __nv_bfloat16* lat = v_l ? p.v_lat : p.k_lat;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) src_l[i] = lat + (at[i] >= 0 ? (at[i] + (int64_t)g * step) * r_l + c8 * 8 : 0);
-    u_l = (v_l ? p.u_v : p.u_k) + ((int64_t)h_l * r_l + t8) * kHeadDim + half * kHalf + c8 * 8;
+__global__ void __launch_bounds__(kThreads, 1)
+    palu_rebuild_kv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                           const __grid_constant__ CUtensorMap tm_uk, const __grid_constant__ CUtensorMap tm_uv,
+                           const __grid_constant__ CUtensorMap tm_ko, const __grid_constant__ CUtensorMap tm_vo, const Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int off_u = p.ring * p.a_bytes, off_out = off_u + p.ring * p.u_bytes,
+            off_table = off_out + p.out_bufs * 8 * kOutBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_table + kTableBytes);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  constexpr int B_AF = 0, B_AE = kMaxRing, B_UF = 2 * kMaxRing, B_UE = 3 * kMaxRing, B_DF = 4 * kMaxRing, B_DE = B_DF + kDBufs,
+                B_TF = B_DE + kDBufs, B_TE = B_TF + 1, B_DRAIN = B_TE + 1, B_COUNT = B_DRAIN + 1;
+  static_assert(B_COUNT * 8 + 16 <= 512, "misc area");
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+  auto wait = [&](uint32_t b, uint32_t ph) -> bool { return mbar_wait(b, ph, s_abort, p.status, p.wait_ns); };
+  auto wait_all = [&](uint32_t b, uint32_t ph) -> bool {
+    if (__all_sync(0xffffffffu, mbar_try(b, ph))) return true;
+    return __all_sync(0xffffffffu, mbar_wait_slow(b, ph, s_abort, p.status, p.wait_ns)) != 0;
   };
-  auto copy_job = [&](int buf) {
-    const int r = R ? R : r_l, ch = r >> 3;
-    const uint32_t dl = sb + buf * stage_sz, ls = lat_stride(r), wl = lat_bytes(r) / 4, dt = dl + t8 * ls + c8 * 16;
-    const uint32_t du = dl + lat_bytes(r) + t8 * kUStride + c8 * 16;
-    if constexpr (R != 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < R / 8; c += 8)
-          if (c + 8 <= R / 8 || c + c8 < R / 8) cp_async16(dt + i * wl + c * 16, src_l[i] + c * 8, at[i] >= 0 ? 16 : 0);
-#pragma unroll
-      for (int k = 0; k < R; k += 16) cp_async16(du + k * kUStride, u_l + k * kHeadDim, 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        for (int c = 0; c + c8 < ch; c += 8) cp_async16(dt + i * wl + c * 16, src_l[i] + c * 8, at[i] >= 0 ? 16 : 0);
-#pragma unroll 4
-      for (int k = 0; k < r; k += 16) cp_async16(du + k * kUStride, u_l + k * kHeadDim, 16);
-    }
-    cp_async_commit();
-    ++h_l;
-    u_l += (R ? R : r_l) * kHeadDim;
-    if (R == 0 && h_l == p.n_kv) {
-      if (!v_l && p.u_v) seek(p.n_kv);
-    } else if (++in_group == gs) {
-      in_group = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (at[i] >= 0) src_l[i] += (int64_t)step * (R ? R : r_l);
-    }
-  };
-
-  float cs[2][8], sn[2][8];  // frequency 32 half + 4 j + lane % 4 of rows lane / 4 and + 8 of the warp's 16 tokens
-  seek(j0);
-  copy_job(0);
-  if (j0 + 1 < j1) copy_job(1);
-  if (j0 < p.n_kv) {
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int t = warp * 16 + (lane >> 2) + 8 * y, pos = pos0 + min(t, count - 1);
-      const int64_t at = (int64_t)pos * kHeadDim + kHalf * half + 2 * (lane & 3);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        cs[y][j] = __ldg(p.cos + at + 8 * j);
-        sn[y][j] = __ldg(p.sin + at + 8 * j);
-      }
-    }
-  }
-  const int64_t dst0 = (tok0 + warp * 16 + (lane >> 3)) * p.n_kv * kHeadDim + half * kHalf + (lane & 7) * 8;
-  const int64_t dst_step = (int64_t)4 * p.n_kv * kHeadDim;
-  int buf = 0;
-  for (int job = j0; job < j1; ++job, buf = buf == kStages - 1 ? 0 : buf + 1) {
-    if (job + 1 < j1) cp_async_wait<1>();
-    else cp_async_wait<0>();
-    __syncthreads();  // this head's copies have landed, and the stage of the head before it is free
-    if (job + 2 < j1) copy_job(buf == 0 ? 2 : buf - 1);
-    const bool is_v = R == 0 && job >= p.n_kv;
-    const int h = is_v ? job - p.n_kv : job, r = R ? R : (is_v ? p.r_v : p.r_k);
-    float acc[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) acc[j][x] = 0.f;
-    const uint32_t sl = sb + buf * stage_sz, su = sl + lat_bytes(r);
-    const uint32_t a_at = sl + warp * (lat_bytes(r) / 4) + (lane & 15) * lat_stride(r) + (lane >> 4) * 16;
-    const uint32_t b_at = su + (lane & 15) * kUStride + (lane >> 4) * 16;
-#pragma unroll(R ? R / 16 : 2)
-    for (int k = 0; k < r; k += 16) {
-      uint32_t a0, a1, a2, a3;
-      ldsm_x4(a_at + k * 2, a0, a1, a2, a3);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t b0, b1, b2, b3;
-        ldsm_x4_t(b_at + k * kUStride + j * 32, b0, b1, b2, b3);
-        mma_bf16(acc[2 * j], a0, a1, a2, a3, b0, b1);
-        mma_bf16(acc[2 * j + 1], a0, a1, a2, a3, b2, b3);
-      }
-    }
-    if (!is_v) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float a = acc[j][2 * y], b = acc[j][2 * y + 1];
-          acc[j][2 * y] = a * cs[y][j] - b * sn[y][j];
-          acc[j][2 * y + 1] = b * cs[y][j] + a * sn[y][j];
+  // the same without a call, for the warps that hold the table's rows in registers
+  auto wait_all_inline = [&](uint32_t b, uint32_t ph) -> bool {
+    bool done = mbar_try(b, ph);
+    if (!done) {
+      const unsigned long long t0 = globaltimer();
+      while (!(done = mbar_try(b, ph))) {
+        if (*s_abort) break;
+        if (globaltimer() - t0 > p.wait_ns) {
+          *s_abort = 1;
+          atomicExch(p.status, kStatusTimeout);
+          break;
         }
-    }
-    // 16 rows of 64 results through shared memory: 8 x 8 blocks (rows 0..7 and 8..15 of columns 8 j, then 8 j + 8)
-    __syncwarp();
-    unsigned char* out = smem + buf * stage_sz + warp * (lat_bytes(r) / 4);
-    const uint32_t so = smem_u32(out) + (lane & 15) * kUStride + (lane >> 4) * 16;
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      uint32_t w[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int jj = j + (x >> 1), y = x & 1;
-        const float a = acc[jj][2 * y], b = acc[jj][2 * y + 1];
-        w[x] = pack_bf16(a, b);
       }
-      stsm_x4(so + j * 16, w[0], w[1], w[2], w[3]);
     }
-    __syncwarp();
-    __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + dst0 + h * kHeadDim;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (warp * 16 + i * 4 + (lane >> 3) < count)
-        *reinterpret_cast<uint4*>(dst + i * dst_step) =
-            *reinterpret_cast<const uint4*>(out + (i * 4 + (lane >> 3)) * kUStride + (lane & 7) * 16);
+    return __all_sync(0xffffffffu, done) != 0;
+  };
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < B_DE; ++i) mbar_init(bar(i), 1);
+    for (int i = 0; i < kDBufs; ++i) mbar_init(bar(B_DE + i), 8);
+    mbar_init(bar(B_TF), 2);
+    mbar_init(bar(B_TE), 8);
+    mbar_init(bar(B_DRAIN), 1);
+    *s_abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *s_tmem;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRoleRegs));
+    if (warp == 8) {
+      if (lane == 0) {
+        // ============================== TMA producer ==============================
+        int na = 0, nu = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+          const int4 tile = p.tiles[u / p.runs];
+          const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
+          for (int job = j0; ok && job < j1; ++job) {
+            const Job x = job_of(p, job, j0, j1);
+            if (x.new_a) {
+              const int s = na % p.ring, use = na / p.ring;
+              if (use >= 1 && !(ok = wait(bar(B_AE + s), (use - 1) & 1))) break;
+              const CUtensorMap* tm = x.is_v ? &tm_v : &tm_k;
+              const int nbox = (x.r + 63) >> 6;
+              const uint32_t dst = sbase + s * p.a_bytes, full = bar(B_AF + s);
+              mbar_expect_tx(full, nbox * kBox);
+              if (!p.page_table) {
+                for (int c = 0; c < nbox; ++c) tma_load_3d(dst + c * kBox, tm, full, c * 64, tile.y, tile.x * p.n_groups + x.g);
+              } else {
+                // one box a page (pages of 2^blk_shift rows; a whole number of swizzle atoms); pages that the table does not
+                // name, and those behind the row, are read past the tensor: zeros
+                const int sub = kTokens >> p.blk_shift, first = tile.y >> p.blk_shift, last = (tile.y + tile.w - 1) >> p.blk_shift;
+                for (int i = 0; i < sub; ++i) {
+                  int b = p.n_blocks;
+                  if (first + i <= last) {
+                    const int e = p.page_table[(int64_t)tile.x * p.table_ld + first + i];
+                    if ((unsigned)e < (unsigned)p.n_blocks) b = e;
+                  }
+                  for (int c = 0; c < nbox; ++c)
+                    tma_load_3d(dst + c * kBox + (i << p.blk_shift) * 128, tm, full, c * 64, 0, b * p.n_groups + x.g);
+                }
+              }
+              ++na;
+            }
+            const int s = nu % p.ring, use = nu / p.ring;
+            if (use >= 1 && !(ok = wait(bar(B_UE + s), (use - 1) & 1))) break;
+            const CUtensorMap* tm = x.is_v ? &tm_uv : &tm_uk;
+            mbar_expect_tx(bar(B_UF + s), x.r * 256);
+            for (int c = 0; c < 2; ++c)
+              tma_load_2d(sbase + off_u + s * p.u_bytes + c * x.r * 128, tm, bar(B_UF + s), c * 64, x.h * x.r);
+            ++nu;
+          }
+        }
+        if (*s_abort) {  // let every copy already issued land before the CTA can exit
+          for (int n = max(0, na - p.ring); n < na; ++n) mbar_drain(bar(B_AF + n % p.ring), (n / p.ring) & 1);
+          for (int n = max(0, nu - p.ring); n < nu; ++n) mbar_drain(bar(B_UF + n % p.ring), (n / p.ring) & 1);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // ============================== MMA issuer ==============================
+      constexpr uint32_t ID = idesc_f16(128, 1, false, true);  // latents (K-major) x U (MN-major)
+      int na = -1, nu = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
+        for (int job = j0; job < j1; ++job) {
+          const Job x = job_of(p, job, j0, j1);
+          na += x.new_a;
+          const int sa = na % p.ring, su = nu % p.ring, d = nu % kDBufs, use = nu / kDBufs;
+          if (x.new_a && !(ok = wait_all(bar(B_AF + sa), (na / p.ring) & 1))) break;
+          if (!(ok = wait_all(bar(B_UF + su), (nu / p.ring) & 1))) break;
+          if (use >= 1 && !(ok = wait_all(bar(B_DE + d), (use - 1) & 1))) break;
+          fence_after();
+          const uint64_t a = sdesc(sbase + sa * p.a_bytes, 16, 1024), b = sdesc(sbase + off_u + su * p.u_bytes, x.r * 128, 1024);
+          if (elect_one()) {
+            for (int kk = 0; kk < x.r >> 4; ++kk)
+              mma_ss(tmem + d * 128, a + (((kk >> 2) * kBox + (kk & 3) * 32) >> 4), b + kk * (2048 >> 4), ID, kk > 0);
+            mma_commit(bar(B_DF + d));
+            mma_commit(bar(B_UE + su));
+            if (x.last_of_a) mma_commit(bar(B_AE + sa));
+          }
+          __syncwarp();
+          ++nu;
+        }
+      }
+      if (elect_one()) mma_commit(bar(B_DRAIN));
+      __syncwarp();
+      mbar_drain(bar(B_DRAIN), 0);
+    } else if (warp >= 10) {
+      // ============================== table ==============================
+      // The next unit's table rows, while its predecessor's heads are worked on: 4-byte copies, which leave out each
+      // frequency's second place; a lane a frequency, 32 of them 128 bytes, whose 16-byte chunk k goes to k ^ (row & 7).
+      const uint32_t table = sbase + off_table + (lane & 3) * 4;
+      int n = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
+        if ((u % p.runs) * p.per_unit >= p.n_kv) continue;  // V heads only
+        const int4 tile = p.tiles[u / p.runs];
+        if (n >= 1 && !(ok = wait_all(bar(B_TE), (n - 1) & 1))) break;
+        ++n;
+#pragma unroll 4
+        for (int r = warp - 10; r < kTokens; r += 2) {
+          const int64_t at = (int64_t)(tile.y + min(r, tile.w - 1)) * kHeadDim + 2 * lane;
+          const uint32_t to = table + r * 512 + (((lane >> 2) ^ (r & 7)) << 4);
+          cp_async4(to, p.cos + at);
+          cp_async4(to + 128, p.cos + at + 64);
+          cp_async4(to + 256, p.sin + at);
+          cp_async4(to + 384, p.sin + at + 64);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_TF));
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kResultRegs));
+    // ============================== results ==============================
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const uint32_t tD = tmem + ((uint32_t)(quarter * 32) << 16) + 64 * half;
+    int nu = 0, n_t = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
+      const int4 tile = p.tiles[u / p.runs];
+      const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
+      float cs[32], sn[32];  // the token's frequencies 32 half .. + 31
+      if (j0 < p.n_kv) {
+        if (ok) ok = wait_all_inline(bar(B_TF), n_t & 1);
+        ++n_t;
+        const unsigned char* at = smem + off_table + row * 512 + half * 128;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 c = *reinterpret_cast<const float4*>(at + ((i ^ (row & 7)) << 4));
+          const float4 s = *reinterpret_cast<const float4*>(at + 256 + ((i ^ (row & 7)) << 4));
+          cs[4 * i] = c.x;
+          cs[4 * i + 1] = c.y;
+          cs[4 * i + 2] = c.z;
+          cs[4 * i + 3] = c.w;
+          sn[4 * i] = s.x;
+          sn[4 * i + 1] = s.y;
+          sn[4 * i + 2] = s.z;
+          sn[4 * i + 3] = s.w;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_TE));
+      }
+      for (int job = j0; job < j1; ++job) {
+        const Job x = job_of(p, job, j0, j1);
+        __nv_bfloat16* dst = (x.is_v ? p.v_out : p.k_out) + ((int64_t)(tile.z + quarter * 32) * p.n_kv + x.h) * kHeadDim + 64 * half;
+        const int64_t step = (int64_t)p.n_kv * kHeadDim;
+        if (ok) {
+          const int d = nu % kDBufs;
+          ok = wait_all_inline(bar(B_DF + d), (nu / kDBufs) & 1);
+          ++nu;
+          if (ok) {
+            fence_after();
+            uint32_t v[64];
+            tmem_ld32p(tD + d * 128, v);
+            tmem_ld32p(tD + d * 128 + 32, v + 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) touch16(v + 16 * i);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(B_DE + d));
+            if (!x.is_v) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
+                v[2 * i] = __float_as_uint(a * cs[i] - b * sn[i]);
+                v[2 * i + 1] = __float_as_uint(b * cs[i] + a * sn[i]);
+              }
+            }
+            // the warp's 32 rows x 128 bytes in the layout that a swizzled TMA store takes; whole blocks of rows go out by TMA,
+            // those that the tile's end cuts by the lanes
+            unsigned char* stage = smem + off_out + ((nu % p.out_bufs) * 8 + warp) * kOutBytes;
+            if (lane == 0) {
+              if (p.out_bufs == 2) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+              else asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+            }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              uint32_t h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) h[q] = pack_bf16(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]));
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            if (quarter * 32 + 32 <= tile.w) {
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0)
+                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(
+                                 reinterpret_cast<uint64_t>(x.is_v ? &tm_vo : &tm_ko)),
+                             "r"(smem_u32(stage)), "r"(64 * half), "r"(x.h), "r"(tile.z + quarter * 32)
+                             : "memory");
+            } else {
+              __syncwarp();
+              const int k = lane & 7;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                if (quarter * 32 + r < tile.w)
+                  *reinterpret_cast<uint4*>(dst + r * step + 8 * k) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
+              }
+              __syncwarp();
+            }
+            if (lane == 0) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");  // one group a head, empty ones among them
+          }
+        }
+        if (!ok && row < tile.w)
+          for (int i = 0; i < 64; ++i) dst[lane * step + i] = __float2bfloat16(NAN);
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+    __syncwarp();
+  }
+  // every role reaches this point warp-converged
+  fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Absorbed V: the cached latents of a tile's tokens as they are, 8 lanes 128 bytes of a token and latent head. A copy: bound by
+// reading and writing it once.
+constexpr int kGatherThreads = 256;
+__global__ void __launch_bounds__(kGatherThreads) palu_gather_latents_kernel(const Params p) {
+  const int4 tile = p.tiles[blockIdx.x];
+  const int t8 = threadIdx.x >> 3, c8 = threadIdx.x & 7, ch = p.r_v >> 3;
+  int64_t at[4];  // cache rows of the tokens t8, t8 + 32, ... for latent head 0; each further head `step` rows on
+  const int step = p.page_table ? 1 << p.blk_shift : p.max_seq;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = t8 + 32 * i, pos = tile.y + t;
+    at[i] = -1;
+    if (t < tile.w) {
+      if (!p.page_table) {
+        at[i] = (int64_t)tile.x * p.n_groups * p.max_seq + pos;
+      } else {
+        const int b = p.page_table[(int64_t)tile.x * p.table_ld + (pos >> p.blk_shift)];
+        if ((unsigned)b < (unsigned)p.n_blocks) at[i] = (((int64_t)b * p.n_groups) << p.blk_shift) + (pos & (step - 1));
+      }
+    }
+  }
+  for (int g = blockIdx.y; g < p.n_groups; g += gridDim.y)
+    for (int c = c8; c < ch; c += 8) {
+      uint4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (at[i] >= 0) v[i] = *reinterpret_cast<const uint4*>(p.v_lat + (at[i] + (int64_t)g * step) * p.r_v + c * 8);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (t8 + 32 * i < tile.w)
+          *reinterpret_cast<uint4*>(p.v_out + ((int64_t)(tile.z + t8 + 32 * i) * p.n_groups + g) * p.r_v + c * 8) = v[i];
+    }
 }
 
 }  // namespace rb
