@@ -136,11 +136,11 @@ def load() -> ctypes.CDLL:
     pool_p, cache_p = ctypes.POINTER(PagePoolInfo), ctypes.POINTER(PageCache)
     lib.palu_page_workspace_bytes.argtypes = [i32]
     lib.palu_page_workspace_bytes.restype = sz
-    lib.palu_reserve_pages.argtypes = [pool_p, i32_p, i32_p, i32, vp]
-    lib.palu_fork_pages.argtypes = [pool_p, cache_p, i32, i32_p, i32_p, i32_p, i32, vp, sz, vp]
-    lib.palu_free_pages.argtypes = [pool_p, i32_p, i32, vp]
+    lib.palu_reserve_pages.argtypes = [pool_p, vp, vp, i32, vp]
+    lib.palu_fork_pages.argtypes = [pool_p, cache_p, i32, vp, vp, vp, i32, vp, sz, vp]
+    lib.palu_free_pages.argtypes = [pool_p, vp, i32, vp]
     lib.palu_compact_pages.argtypes = [pool_p, cache_p, i32, vp, sz, vp]
-    lib.palu_copy_pages.argtypes = [cache_p, i32, i32, i32_p, i32_p, i32, vp]
+    lib.palu_copy_pages.argtypes = [cache_p, i32, i32, vp, vp, i32, vp]
     for f in ("reserve", "fork", "free", "compact", "copy"):
         getattr(lib, f"palu_{f}_pages").restype = ctypes.c_int
     lib.palu_last_error.argtypes = []

@@ -8,6 +8,7 @@ reference plans paged caches and has not built them (HANDOFF.md:54-55, 126-127).
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Sequence
 
 import torch
@@ -18,14 +19,20 @@ STATUS = {1: "the pool ran out of pages", 2: "a fork's parent held fewer positio
           4: "a fork's child was not empty"}
 
 
-def _ints(x, what: str):
+def _ints(x, what: str) -> array:
+    """Host integers as a C int array (``_at`` is its address)."""
     if isinstance(x, torch.Tensor):
         if x.is_cuda:
             raise RuntimeError(f"{what} must be on the host (a sequence or a CPU tensor)")
         x = x.reshape(-1).tolist()
-    if any(not -2**31 <= v < 2**31 for v in x):
-        raise RuntimeError(f"{what} must fit 32 bits")
-    return (ctypes.c_int32 * len(x))(*x)
+    try:
+        return array("i", x)
+    except OverflowError:
+        raise RuntimeError(f"{what} must fit 32 bits") from None
+
+
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _caches(caches: Sequence[torch.Tensor]):
@@ -54,7 +61,7 @@ def copy_pages(caches: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence
     if len(s) != len(d):
         raise RuntimeError(f"src and dst must have the same length, got {len(s)} and {len(d)}")
     with torch.cuda.device(device):
-        _lib.check(_lib.load().palu_copy_pages(arr, len(arr), n_blocks, s, d, len(s), _lib.stream_handle(device)))
+        _lib.check(_lib.load().palu_copy_pages(arr, len(arr), n_blocks, _at(s), _at(d), len(s), _lib.stream_handle(device)))
 
 
 class PagePool:
@@ -85,6 +92,7 @@ class PagePool:
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         lib = _lib.load()
         self._ws = torch.empty(int(lib.palu_page_workspace_bytes(self.n_blocks)), dtype=torch.uint8, device=self.device)
+        self._ws_at, self._ws_bytes, self._n_caches = self._ws.data_ptr(), self._ws.numel(), len(self._caches)
         self._pool = ctypes.byref(_lib.PagePoolInfo(self.table.data_ptr(), self.refs.data_ptr(), self.mapped.data_ptr(),
                                                     self._status.data_ptr(), self.rows, self.blocks_per_row, self.n_blocks,
                                                     self.block_size))
@@ -100,7 +108,7 @@ class PagePool:
         r, n = _ints(rows, "rows"), _ints(lens, "lens")
         if len(r) != len(n):
             raise RuntimeError(f"rows and lens must have the same length, got {len(r)} and {len(n)}")
-        self._call(_lib.load().palu_reserve_pages, r, n, len(r))
+        self._call(_lib.load().palu_reserve_pages, _at(r), _at(n), len(r))
 
     def fork(self, parents: Sequence[int], children: Sequence[int], lens: Sequence[int]) -> None:
         """children[i], an empty row, continues parents[i] behind its first lens[i] positions (palu_fork_pages): whole pages
@@ -108,17 +116,17 @@ class PagePool:
         p, c, n = _ints(parents, "parents"), _ints(children, "children"), _ints(lens, "lens")
         if not len(p) == len(c) == len(n):
             raise RuntimeError(f"parents, children and lens must have the same length, got {len(p)}, {len(c)} and {len(n)}")
-        self._call(_lib.load().palu_fork_pages, self._caches, len(self._caches), p, c, n, len(p), self._ws.data_ptr(),
-                   self._ws.numel())
+        self._call(_lib.load().palu_fork_pages, self._caches, self._n_caches, _at(p), _at(c), _at(n), len(p), self._ws_at,
+                   self._ws_bytes)
 
     def free(self, rows: Sequence[int]) -> None:
         """The rows give up their pages (palu_free_pages); a page is free once no row names it."""
         r = _ints(rows, "rows")
-        self._call(_lib.load().palu_free_pages, r, len(r))
+        self._call(_lib.load().palu_free_pages, _at(r), len(r))
 
     def compact(self) -> None:
         """Pages in use move to the lowest places, in every cache; table and counts follow (palu_compact_pages)."""
-        self._call(_lib.load().palu_compact_pages, self._caches, len(self._caches), self._ws.data_ptr(), self._ws.numel())
+        self._call(_lib.load().palu_compact_pages, self._caches, self._n_caches, self._ws_at, self._ws_bytes)
 
     def check(self) -> None:
         """Wait, and raise RuntimeError for what went wrong in a call since the last check (pages ran out, a fork's parent

@@ -70,6 +70,7 @@ class PrefillPlan:
         _lib.check(st)
         self.q_tokens, self.k_tokens = int(self.info.q_tokens), int(self.info.k_tokens)
         self.n_q_heads, self.n_kv_heads = int(n_q_heads), int(n_kv_heads)
+        self.max_k_len, self.max_row = int(self.info.max_k_len), int(self.info.max_row)
         self._ws_bytes, self._index = {}, None
         self.host = host[:int(self.info.bytes)]
         self.data = self.host.to(self.device)
@@ -168,46 +169,52 @@ def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor
     [rows, blocks per row] int32 (an entry outside the cache reads as zero latents); u_k [n_kv, r_k, 128], u_v [n_kv, r_v,
     128] bf16; cos / sin [>= longest k_len, 128] fp32 as the layer's tables. Sequence s reads cache row ``plan.rows[s]``.
     fp32 accumulation and rotation, one rounding to bf16."""
-    _lib.require_cuda(k_latent, v_latent, u_k, cos, sin, u_v, page_table)
-    for t, what in ((k_latent, "k_latent"), (v_latent, "v_latent"), (u_k, "u_k"), (cos, "cos"), (sin, "sin"), (u_v, "u_v"),
-                    (page_table, "page_table")):
-        if t is not None and t.device != plan.device:
-            raise RuntimeError(f"{what} is on {t.device}, the plan on {plan.device}")
-    for t, what in ((k_latent, "k_latent"), (v_latent, "v_latent"), (u_k, "u_k"), (u_v, "u_v")):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise RuntimeError(f"{what} must be bf16, got {t.dtype}")
-    if k_latent.dim() != 4 or v_latent.dim() != 4 or k_latent.shape[:3] != v_latent.shape[:3]:
-        raise RuntimeError(f"k_latent and v_latent must be [B, n_groups, S, r] with the same leading dims, got "
-                           f"{tuple(k_latent.shape)} and {tuple(v_latent.shape)}")
-    n_groups, S, r_k, r_v = k_latent.shape[1], k_latent.shape[2], k_latent.shape[3], v_latent.shape[3]
-    n_kv = plan.n_kv_heads
-    if tuple(u_k.shape) != (n_kv, r_k, HEAD_DIM):
-        raise RuntimeError(f"u_k must be [{n_kv}, {r_k}, 128], got {tuple(u_k.shape)}")
+    dev, n_kv = plan.device, plan.n_kv_heads
+    for t, what, dtype in ((k_latent, "k_latent", torch.bfloat16), (v_latent, "v_latent", torch.bfloat16),
+                           (u_k, "u_k", torch.bfloat16), (u_v, "u_v", torch.bfloat16), (cos, "cos", torch.float32),
+                           (sin, "sin", torch.float32), (page_table, "page_table", None)):
+        if t is not None and t.device != dev:
+            _lib.require_cuda(t)
+            raise RuntimeError(f"{what} is on {t.device}, the plan on {dev}")
+        if t is not None and dtype is not None and t.dtype != dtype:
+            raise RuntimeError(f"{what} must be {'fp32' if dtype == torch.float32 else 'bf16'}, got {t.dtype}")
+    ks, vs, us = k_latent.shape, v_latent.shape, u_k.shape
+    if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3]:
+        raise RuntimeError(f"k_latent and v_latent must be [B, n_groups, S, r] with the same leading dims, got {tuple(ks)} and "
+                           f"{tuple(vs)}")
+    rows, n_groups, S, r_k = ks
+    r_v = vs[3]
+    if len(us) != 3 or us[0] != n_kv or us[1] != r_k or us[2] != HEAD_DIM:
+        raise RuntimeError(f"u_k must be [{n_kv}, {r_k}, 128], got {tuple(us)}")
     if u_v is not None and tuple(u_v.shape) != (n_kv, r_v, HEAD_DIM):
         raise RuntimeError(f"u_v must be [{n_kv}, {r_v}, 128], got {tuple(u_v.shape)}")
-    longest, last_row = int(plan.info.max_k_len), int(plan.info.max_row)
-    for t, what in ((cos, "cos"), (sin, "sin")):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != HEAD_DIM or t.shape[0] < longest or not t.is_contiguous():
-            raise RuntimeError(f"{what} must be a contiguous fp32 [>= {longest}, 128] table, got {t.dtype} {tuple(t.shape)}")
-    rows, pg = k_latent.shape[0], None
+    longest, last_row = plan.max_k_len, plan.max_row
+    for t in (cos, sin):
+        if t.dim() != 2 or t.shape[1] != HEAD_DIM or t.shape[0] < longest or not t.is_contiguous():
+            raise RuntimeError(f"cos and sin must be contiguous fp32 [>= {longest}, 128] tables, got {tuple(t.shape)}")
+    pg = None
     if page_table is not None:
-        page_table = page_table.to(torch.int32)
-        page_table = page_table if page_table.stride(-1) == 1 else page_table.contiguous()
-        rows, S = page_table.shape[0], page_table.shape[1] * k_latent.shape[2]
-        pg = ctypes.byref(_lib.pages(page_table, k_latent.shape[2], k_latent.shape[0]))
+        if page_table.dtype != torch.int32 or page_table.stride(-1) != 1:
+            page_table = page_table.to(torch.int32).contiguous()
+        pg = _lib.pages(page_table, S, rows)
+        rows, S = page_table.shape[0], page_table.shape[1] * S
     if longest > S or last_row >= rows:
         raise RuntimeError(f"the plan's longest sequence ({longest}) and last cache row ({last_row}) must fit the {rows} rows of "
                            f"{S} positions")
-    if k_latent.device.index != torch.cuda.current_device():
-        with torch.cuda.device(k_latent.device):
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
             return rebuild_kv(k_latent, v_latent, u_k, cos, sin, plan, u_v=u_v, page_table=page_table)
     k_latent, v_latent, u_k = k_latent.contiguous(), v_latent.contiguous(), u_k.contiguous()
-    u_v = u_v.contiguous() if u_v is not None else None
-    k = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=k_latent.device)
-    v = torch.empty(plan.k_tokens, *((n_kv, HEAD_DIM) if u_v is not None else (n_groups, r_v)), dtype=torch.bfloat16, device=k.device)
-    stream = _lib.stream_handle(k.device)
+    k = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    if u_v is not None:
+        u_v = u_v.contiguous()
+        v = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    else:
+        v = torch.empty(plan.k_tokens, n_groups, r_v, dtype=torch.bfloat16, device=dev)
+    stream = _lib.stream_handle(dev)
     plan.use_on(stream)
     _lib.check(_lib.load().palu_rebuild_kv(
-        k_latent.data_ptr(), v_latent.data_ptr(), u_k.data_ptr(), _lib.ptr(u_v), cos.data_ptr(), sin.data_ptr(), pg,
-        plan.info_ptr, plan.data_ptr, k.data_ptr(), v.data_ptr(), n_groups, r_k, r_v, S, stream))
+        k_latent.data_ptr(), v_latent.data_ptr(), u_k.data_ptr(), None if u_v is None else u_v.data_ptr(), cos.data_ptr(),
+        sin.data_ptr(), None if pg is None else ctypes.byref(pg), plan.info_ptr, plan.data_ptr, k.data_ptr(), v.data_ptr(), n_groups,
+        r_k, r_v, S, stream))
     return k, v
