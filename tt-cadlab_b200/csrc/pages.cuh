@@ -19,6 +19,9 @@ constexpr int kMaxCaches = 128;   // caches of one copy launch
 constexpr int kMaxCopies = 480;   // host-given page copies of one launch
 constexpr int kCopyThreads = 256;
 constexpr int kPart = 16384;      // bytes of a page that a CTA copies at a time
+// CTAs an SM over all caches, at most: small ones that the scheduler deals out as SMs come free. 126 of 512 pages in 64 caches
+// (1.06 GB moved), us, with 8 / 16 / 64 / 128 / 512: 192, 179, 172, 169, 167 (161 at the measured copy rate).
+constexpr int kCopyCtas = 128;
 
 enum : int { kErrFull = 1, kErrParent = 2, kErrChild = 4 };
 

@@ -205,10 +205,10 @@ bool fill_caches(const palu_page_cache* caches, int n, palu::pg::Caches& a, int6
   }
   return wide;
 }
-// Thread blocks per cache: enough for 8 of 256 threads on every SM over all caches, no more than there are units.
+// Thread blocks per cache: kCopyCtas for every SM over all caches, no more than there are units.
 int copy_grid(int n_caches, int64_t moves, int64_t most) {
   const int64_t units = moves * ((most + palu::pg::kPart - 1) / palu::pg::kPart);
-  const int64_t fill = (8LL * device_sms() + n_caches - 1) / std::max(1, n_caches);
+  const int64_t fill = ((int64_t)palu::pg::kCopyCtas * device_sms() + n_caches - 1) / std::max(1, n_caches);
   return (int)std::max<int64_t>(1, std::min(units, fill));
 }
 
