@@ -13,12 +13,22 @@
 // CTAs are persistent. A piece that is not a whole item writes a partial record (O, m, l) that the merge joins.
 // Per key tile t of 128 keys and chain c:
 //   MMA      S_c[128 x 128] (f32, TMEM) = Q_c (smem) x K_t^T (smem), 8 steps of K = 16
-//   softmax  one thread per row: row maximum, exp2, P_c (bf16) -> TMEM; O_c is rescaled only when a row's maximum
-//            outgrew its reference by more than 2^8 (any reference within that keeps P and l in range; the final
-//            division cancels it)
+//   softmax  one thread per row: exp2 against the reference, P_c (bf16) -> TMEM. The reference is the maximum of the row's
+//            first 32 keys and moves (rescaling O_c and l) only when the tile's sum shows that a score may have outgrown
+//            it by 2^9 or more: any reference within that keeps P and l in range, and the final division cancels it. So
+//            no exponential waits for a maximum.
 //   MMA      O_c[128 x d_v] (f32, TMEM) += P_c (TMEM) x V_t (smem, MN-major: as TMA wrote it)
-// The chains run half a period apart: while the tensor cores work on one chain's PV and next S, the other chain's
-// softmax warps exponentiate. Values at most 64 wide leave TMEM columns for P of its own; wider ones write P over S.
+// The chains run half a period apart: while the tensor cores work on one chain's PV and next S, the other chain's softmax
+// warps exponentiate. Values at most 64 wide leave TMEM columns for P of its own, and the next S does not wait for PV; wider
+// ones write P over S.
+//
+// What bounds it: at d_v 128 a tile and chain takes the tensor cores 1290 cycles (16 MMAs; S alone 700, its operands' 64 KB
+// being what shared memory delivers in 512) and the softmax warps 1870 (128 exponentials of the special-function unit a row
+// are 1024), one behind the other: 3230 a tile for both chains, against 2580 if the tensor cores never waited. Measured, 32
+// query and 8 KV heads: 32768 tokens, d_v 128 7.7 ms (1140 TFLOP/s, under the power cap); 8192 tokens 470 us (1170); d_v 64
+// 429 us (960). Tried and not kept: a polynomial for every second to eighth exponential (no faster at any share: the chain's
+// latency is what counts), S in two halves of 64 keys so that the upper one need not wait for PV (9.2 ms: an MMA takes its 64
+// cycles at N = 64 too).
 //
 // Masked places hold anything. Scores behind a row's last visible key are replaced, never added to. V rows behind the
 // item's last visible key are zeroed in shared memory before the product, and non-finite values in the V rows that
