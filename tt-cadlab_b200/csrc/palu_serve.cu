@@ -389,8 +389,11 @@ int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* 
   };
   if (int st = d_v > 64 ? launch(std::true_type{}) : launch(std::false_type{})) return st;
   if (plan->n_merges > 0) {
-    palu::pf::palu_prefill_merge_kernel<<<dim3(plan->n_merges, 8), 256, 0, stream>>>(
-        reinterpret_cast<const palu::pf::PfMerge*>(data + plan->off_merges), p);
+    const auto* merges = reinterpret_cast<const palu::pf::PfMerge*>(data + plan->off_merges);
+    if (plan->n_slots >= palu::pf::kDeepRecords * plan->n_merges)
+      palu::pf::palu_prefill_merge_deep_kernel<<<dim3(plan->n_merges, 8, (d_v + 31) / 32), 256, 0, stream>>>(merges, p);
+    else
+      palu::pf::palu_prefill_merge_kernel<<<dim3(plan->n_merges, 8), 256, 0, stream>>>(merges, p);
     return cuda_check("prefill merge launch");
   }
   return PALU_OK;

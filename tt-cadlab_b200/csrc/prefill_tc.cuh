@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
 // Joins the records of the items that were cut along the keys: with w_s = 2^(m_s - max m),
 // o = sum_s w_s O_s / sum_s w_s l_s. A block joins 32 rows (a lane a row, a warp every eighth column) and writes them
-// through shared memory. Bound by reading the records (fp32).
+// through shared memory. For few records an item, whose loads it issues record by record.
 __global__ void __launch_bounds__(256) palu_prefill_merge_kernel(const PfMerge* merges, const PfParams p) {
   __shared__ float s_o[32][129];
   const PfMerge w = merges[blockIdx.x];
@@ -773,6 +773,63 @@ __global__ void __launch_bounds__(256) palu_prefill_merge_kernel(const PfMerge* 
     if (pos >= p.ppt || lp >= w.npos) continue;
     *reinterpret_cast<uint32_t*>(p.out + (((size_t)w.q0 + lp) * p.n_q + w.kvh * p.rep + row2 % p.rep) * p.dv + 2 * x) =
         pack_bf16(s_o[rr][2 * x], s_o[rr][2 * x + 1]);
+  }
+}
+
+// The same for many records an item (few queries on many keys): a block joins 32 rows of 32 columns, its 8 warps take the
+// records in turn, all of a record's loads at once, and meet in shared memory. Bound by latency. us, with this kernel and with
+// the one above: 64 queries on 32768 keys (19 records) 64 and 69; 512 on 8192 (3 records) 77 and 66: from 8 records on.
+constexpr int kDeepRecords = 8;
+__global__ void __launch_bounds__(256) palu_prefill_merge_deep_kernel(const PfMerge* merges, const PfParams p) {
+  __shared__ float s_o[8][32][33], s_l[8][32];
+  const PfMerge w = merges[blockIdx.x];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = (int)blockIdx.y >> 2, row0 = (int)(blockIdx.y & 3) * 32, row = row0 + lane, x0 = blockIdx.z * 32;
+  if (c * p.ppt + row0 / p.rep >= w.npos) return;  // the block's first row is behind the item
+  const int pos = row / p.rep, lpos = c * p.ppt + pos;
+  const bool have = pos < p.ppt && lpos < w.npos;
+  const float* ml = p.ws_ml + ((size_t)w.slot0 * 2 * kRows + c * kRows + row) * 2;
+  float m = -INFINITY;
+  bool lost = false;
+#pragma unroll 4
+  for (int s = 0; s < w.n; ++s) {
+    const float ms = have ? ml[(size_t)s * 4 * kRows] : -INFINITY;
+    lost |= isnan(ms);
+    m = fmaxf(m, ms);
+  }
+  float l = 0.f, o[32];
+#pragma unroll
+  for (int y = 0; y < 32; ++y) o[y] = 0.f;
+  for (int s = warp; s < w.n; s += 8) {
+    const float ms = have ? ml[(size_t)s * 4 * kRows] : -INFINITY;
+    if (ms == -INFINITY) continue;  // the row saw nothing of this piece
+    const float wt = fast_exp2(ms - m);
+    l += wt * ml[(size_t)s * 4 * kRows + 1];
+    const float* po = p.ws_o + (((size_t)(w.slot0 + s) * 2 + c) * p.dv + x0) * kRows + row;
+#pragma unroll
+    for (int y = 0; y < 32; ++y)
+      if (x0 + y < p.dv) o[y] += wt * po[y * kRows];
+  }
+#pragma unroll
+  for (int y = 0; y < 32; ++y) s_o[warp][lane][y] = o[y];
+  s_l[warp][lane] = l;
+  __syncthreads();
+  // a warp writes 4 rows: sums over the warps' parts, 8 lanes a row, 4 columns a lane
+  const int r = warp * 4 + (lane >> 3), y0 = (lane & 7) * 4;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f}, total = 0.f;
+#pragma unroll
+  for (int x = 0; x < 8; ++x) {
+    total += s_l[x][r];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) sum[y] += s_o[x][r][y0 + y];
+  }
+  const bool bad = __shfl_sync(0xffffffffu, (int)lost, r) != 0;
+  const int rpos = (row0 + r) / p.rep, rl = c * p.ppt + rpos;
+  if (rpos < p.ppt && rl < w.npos && x0 + y0 < p.dv) {
+    const float inv = bad ? NAN : 1.f / total;
+    const bool empty = w.vis0 + rl <= 0;
+    const uint2 h = empty ? make_uint2(0u, 0u) : make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
+    *reinterpret_cast<uint2*>(p.out + (((size_t)w.q0 + rl) * p.n_q + w.kvh * p.rep + (row0 + r) % p.rep) * p.dv + x0 + y0) = h;
   }
 }
 
