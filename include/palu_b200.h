@@ -304,7 +304,7 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
  * head strides in elements (multiples of 8; the last dimension is contiguous; 16-byte aligned); out
  * [q_tokens][n_q_heads][d_v] bf16, contiguous. d_v a multiple of 16 in [16, 128]. scale > 0. plan_data: the plan's
  * buffer on the device. workspace: palu_prefill_workspace_bytes(plan, d_v) bytes (0 for most plans; the partial
- * results of work that was split along the keys), not shared by calls that overlap in time. A bounded device wait that
+ * results of work that was split along the keys), not shared by calls that overlap in time. out overlaps no input. A bounded device wait that
  * expires sets the plan's status word, and the rows that it kept from being computed are NaN.
  */
 size_t palu_prefill_workspace_bytes(const palu_prefill_plan* plan, int32_t d_v);

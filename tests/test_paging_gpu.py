@@ -205,3 +205,20 @@ def test_compacting_an_empty_and_a_full_pool(cuda):
     model.reserve([3], [96])
     pool.compact()
     compare(pool, model, caches, plain)
+
+
+def test_lengths_near_the_end_of_32_bits(cuda):
+    """Blocks of 2^30 positions (no cache is named, so nothing has their size): the last lengths that 32 bits hold."""
+    import ctypes
+    from palu_b200 import _lib
+    lib, n = _lib.load(), 4
+    state = torch.tensor([-1] * 4 + [0] * n + [0] * 2 + [0], dtype=torch.int32, device=cuda)   # table [2][2], refs, mapped, status
+    at = lambda i: state.data_ptr() + 4 * i
+    pool = ctypes.byref(_lib.PagePoolInfo(at(0), at(4), at(4 + n), at(6 + n), 2, 2, n, 1 << 30))
+    ints = lambda *x: (ctypes.c_int32 * len(x))(*x)
+    ws = torch.zeros(int(lib.palu_page_workspace_bytes(n)), dtype=torch.uint8, device=cuda)
+    most = 2**31 - 1
+    _lib.check(lib.palu_reserve_pages(pool, ints(0), ints(most), 1, None))
+    _lib.check(lib.palu_fork_pages(pool, None, 0, ints(0), ints(1), ints(most), 1, ws.data_ptr(), ws.numel(), None))
+    torch.cuda.synchronize()
+    assert state.tolist() == [0, 1, 0, 2, 2, 1, 1, 0, 2, 2, 0]     # the child shares page 0 and has a page of its own

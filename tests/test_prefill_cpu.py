@@ -130,3 +130,10 @@ def test_cpu_tensors_are_refused():
     q = torch.zeros(4, 4, 128, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         prefill.prefill_attn(q, q, q, None)
+
+
+def test_limits_of_the_largest_calls():
+    with pytest.raises(RuntimeError, match="work items"):
+        plan([1 << 28], [1], 1024, 8)                     # 2^27 query tiles x 8 KV heads
+    st, msg = _call(plan([4], [4], 4, 1)[0], scale=3e38)  # finite, but not times log2 e
+    assert st == _lib.PALU_ERR_INVALID and "scale" in msg

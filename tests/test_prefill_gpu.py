@@ -224,3 +224,44 @@ def test_empty_batches(cuda):
     assert attend(cuda, q, k, v, [0, 0], [0, 7]).shape == (0, 4, 64)
     q, k, v = inputs([3], [0], 4, 2, 64)
     assert (attend(cuda, q, k, v, [3], [0]) == 0).all()
+
+
+def test_out_must_not_overlap_the_inputs(cuda):
+    from palu_b200 import prefill
+    q, k, v = (t.to(cuda) for t in inputs([40], [40], 2, 2, 128))
+    plan = prefill.PrefillPlan([40], n_q_heads=2, n_kv_heads=2, device=cuda)
+    for out in (q, k, v):
+        with pytest.raises(RuntimeError, match="overlap"):
+            prefill.prefill_attn(q, k, v, plan, out=out)
+    room = torch.empty(2, 40, 2, 128, dtype=torch.bfloat16, device=cuda)  # neighbours are fine
+    room[0] = q
+    assert torch.equal(prefill.prefill_attn(room[0], k, v, plan, out=room[1]), prefill.prefill_attn(q, k, v, plan))
+
+
+def test_a_plan_made_on_another_stream(cuda):
+    """The plan, and its token index, are used on a stream other than the one they were made on and then dropped."""
+    from palu_b200 import prefill
+    q, k, v = (t.to(cuda) for t in inputs([300, 7], [300, 90], 4, 2, 64))
+    side = torch.cuda.Stream()
+    plan = prefill.PrefillPlan([300, 7], [300, 90], rows=[3, 1], n_q_heads=4, n_kv_heads=2, device=cuda)
+    want = prefill.prefill_attn(q, k, v, plan)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        rows, pos = plan.token_index()
+        got = prefill.prefill_attn(q, k, v, plan)
+        where = torch.stack([rows, pos])
+        del plan, rows, pos
+    full = torch.full((1 << 16,), -1, dtype=torch.int32, device=cuda)     # reuses the freed memory where it may
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and int(full.max()) == -1
+    assert torch.equal(where.cpu(), torch.stack([torch.tensor([3] * 300 + [1] * 7), torch.tensor([*range(300), *range(83, 90)])]))
+
+
+def test_token_index_is_not_laid_out_in_a_capture(cuda):
+    from palu_b200 import prefill
+    plan = prefill.PrefillPlan([3], n_q_heads=4, n_kv_heads=2, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        torch.zeros(1, device=cuda)
+        with pytest.raises(RuntimeError, match="before capturing"):
+            plan.token_index()

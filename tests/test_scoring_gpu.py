@@ -207,3 +207,10 @@ def test_many_equal_elements_at_the_border_of_the_top(cuda):
         logits[:, vocab // 3] = 2.0
         logits[n // 2, :vocab // 2] = 0.5
         check(cuda, logits, torch.zeros(n, dtype=torch.long, device=cuda), 9)
+
+
+def test_a_vocabulary_past_32_bits_is_refused(cuda):
+    from palu_b200 import scoring
+    logits = torch.zeros(1, 1, dtype=torch.bfloat16, device=cuda).expand(1, 2**31)
+    with pytest.raises(RuntimeError, match="vocab"):
+        scoring.token_logprobs(logits, torch.zeros(1, dtype=torch.long, device=cuda))

@@ -55,7 +55,7 @@ def pool(**kw):
 CACHE = (_lib.PageCache * 1)(_lib.PageCache(16, 64, 64))
 
 
-@pytest.mark.parametrize("p,needle", [(dict(table=None), "must be set"), (dict(status=None), "must be set"), (dict(rows=0), "positive"),
+@pytest.mark.parametrize("p,needle", [(dict(table=None), "must be set"), (dict(status=None), "must be set"), (dict(rows=0), "positive"), (dict(rows=1 << 16, blocks_per_row=1 << 15), "entries"),
                                       (dict(block_size=-1), "positive")])
 def test_pool_refusals(lib, p, needle):
     for st in (lib.palu_reserve_pages(pool(**p), arr(0), arr(1), 1, None), lib.palu_free_pages(pool(**p), arr(0), 1, None),

@@ -160,3 +160,11 @@ def test_decode_logprobs(cuda):
 def test_page_pool_needs_paged_caches(cuda):
     with pytest.raises(RuntimeError, match="paged"):
         make_decoder(cuda, False).page_pool(2)
+
+
+def test_a_batch_without_tokens(cuda):
+    m = make_decoder(cuda, False)
+    none, plan = torch.zeros(0, dtype=torch.long), m.prefill_plan([0, 0])
+    assert m.prefill_packed(none, plan).shape == (0, 512) and m.prefill_packed_logits(none, plan).shape == (0, 301)
+    got = m.score(none, plan, top=2)
+    assert got.logprob.shape == (0,) and got.top_id.shape == (0, 2)

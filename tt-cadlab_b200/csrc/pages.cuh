@@ -90,6 +90,9 @@ PALU_DEVINL int take_free(const Pool& p, int want, int* s_warp, Take take) {
   return min(found, want);
 }
 
+// Pages of `len` positions (len + size - 1 need not fit 32 bits).
+PALU_DEVINL int pages_of(int len, int size) { return len / size + (len % size != 0); }
+
 struct RowLens {
   int n;
   int32_t row[kMaxPairs], len[kMaxPairs];
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(kPlanThreads) palu_reserve_pages_kernel(const 
   if (threadIdx.x < a.n) {
     const int have = p.mapped[a.row[threadIdx.x]];
     s_have[threadIdx.x] = have;
-    need = max(0, (a.len[threadIdx.x] + p.page_size - 1) / p.page_size - have);
+    need = max(0, pages_of(a.len[threadIdx.x], p.page_size) - have);
   }
   int total;
   const int at = block_scan(need, s_warp, total);
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kPlanThreads) palu_fork_pages_kernel(const Poo
   int need = 0;
   bool ok = false;
   if (i < a.n) {
-    const int full = a.len[i] / p.page_size, count = (a.len[i] + p.page_size - 1) / p.page_size;
+    const int full = a.len[i] / p.page_size, count = pages_of(a.len[i], p.page_size);
     ok = true;
     if (p.mapped[a.parent[i]] < count) {
       atomicOr(p.status, kErrParent);

@@ -2,7 +2,7 @@
 // dispatch on the host; the kernels live in the .cuh files next to it.
 #include <algorithm>
 #include <atomic>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "../../include/palu_b200.h"
@@ -167,6 +167,7 @@ int check_pool(const palu_page_pool* q, palu::pg::Pool& p) {
   if (q->rows <= 0 || q->blocks_per_row <= 0 || q->n_blocks <= 0 || q->block_size <= 0)
     return fail(PALU_ERR_INVALID, "pool: rows, blocks_per_row, n_blocks and block_size must be positive (got %d, %d, %d, %d)", q->rows,
                 q->blocks_per_row, q->n_blocks, q->block_size);
+  if ((int64_t)q->rows * q->blocks_per_row > INT32_MAX) return fail(PALU_ERR_INVALID, "pool: a table of more than 2^31 - 1 entries");
   p = {q->table, q->refs, q->mapped, q->status, q->rows, q->blocks_per_row, q->n_blocks, q->block_size};
   return PALU_OK;
 }
@@ -244,14 +245,14 @@ int apply_moves(const palu::pg::Pool& p, const palu::pg::Moves& mv, const int32_
   return PALU_OK;
 }
 
-// Runs f and turns a C++ exception (out of host memory) into a status.
+// Runs f and turns a C++ exception (all that can throw is a list's allocation) into a status.
 template <class F>
 int guarded(F f) {
   g_err.clear();
   try {
     return f();
-  } catch (const std::bad_alloc&) {
-    return fail(PALU_ERR_INVALID, "out of host memory");
+  } catch (const std::exception& e) {
+    return fail(PALU_ERR_INVALID, "out of host memory (%s)", e.what());
   }
 }
 
@@ -269,18 +270,21 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
   const int rep = n_q_heads / n_kv_heads;
   if (rep > palu::pf::kRows) return fail(PALU_ERR_INVALID, "at most 128 query heads per KV head are supported, got %d", rep);
   if (n_ctas < 0 || n_ctas > 4096) return fail(PALU_ERR_INVALID, "n_ctas must be in [0, 4096], got %d", n_ctas);
-  int64_t tq = 0, tk = 0;
+  int64_t tq = 0, tk = 0, items = 0;
+  const int step = 2 * (palu::pf::kRows / rep);  // query positions of a work item
   int32_t longest = 0, last_row = -1;
   for (int s = 0; s < n_seq; ++s) {
     if (q_lens[s] < 0 || k_lens[s] < 0)
       return fail(PALU_ERR_INVALID, "sequence %d: lengths must not be negative (got %d queries, %d keys)", s, q_lens[s], k_lens[s]);
     if (rows && rows[s] < 0) return fail(PALU_ERR_INVALID, "sequence %d: cache row %d is negative", s, rows[s]);
     tq += q_lens[s];
+    items += (q_lens[s] + (int64_t)step - 1) / step;
     tk += k_lens[s];
     longest = std::max(longest, k_lens[s]);
     last_row = std::max(last_row, rows ? rows[s] : s);
   }
   if (tq > (1 << 28) || tk > (1 << 28)) return fail(PALU_ERR_INVALID, "at most 2^28 packed tokens are supported");
+  if (items * n_kv_heads > (1 << 28)) return fail(PALU_ERR_INVALID, "at most 2^28 work items (query tiles x KV heads) are supported");
   try {
     Lists l;
     const int ppt = palu::pf::kRows / rep;
@@ -313,8 +317,8 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
     std::copy(l.merges.begin(), l.merges.end(), reinterpret_cast<palu::pf::PfMerge*>(b + plan->off_merges));
     std::copy(l.tiles.begin(), l.tiles.end(), reinterpret_cast<int4*>(b + plan->off_tiles));
     return PALU_OK;
-  } catch (const std::bad_alloc&) {
-    return fail(PALU_ERR_INVALID, "out of host memory while planning");
+  } catch (const std::exception& e) {
+    return fail(PALU_ERR_INVALID, "out of host memory while planning (%s)", e.what());
   }
 }
 
@@ -328,7 +332,7 @@ int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* 
   g_err.clear();
   if (!plan || !plan_data) return fail(PALU_ERR_INVALID, "prefill: plan and its device data must be set");
   if (d_v < 16 || d_v > 128 || d_v % 16 != 0) return fail(PALU_ERR_INVALID, "d_v must be a multiple of 16 in [16, 128], got %d", d_v);
-  if (!(scale > 0.f) || !(scale < INFINITY)) return fail(PALU_ERR_INVALID, "scale must be positive and finite");
+  if (!(scale > 0.f) || !(scale * palu::kLog2e < INFINITY)) return fail(PALU_ERR_INVALID, "scale must be positive and finite (also times log2 e)");
   if (plan->q_tokens == 0) return PALU_OK;
   if (!q || !out || (plan->k_tokens > 0 && (!k || !v))) return fail(PALU_ERR_INVALID, "prefill: q, k, v and out must be set");
   auto aligned = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };

@@ -260,7 +260,7 @@ class PaluDecoder:
         without a token have no row)."""
         x = self.prefill_packed(tokens, plan, page_table)
         lens = [n for n in plan.q_lens if n]
-        last = (torch.tensor(lens).cumsum(0) - 1).to(self.device)
+        last = (torch.tensor(lens, dtype=torch.int64).cumsum(0) - 1).to(self.device)
         return (x[last] @ self.lm_head.t()).float()
 
     @torch.no_grad()
@@ -272,7 +272,7 @@ class PaluDecoder:
         x = self.prefill_packed(tokens, plan, page_table)
         nxt = torch.full((plan.q_tokens,), -1, dtype=torch.int64, device=self.device)
         nxt[:-1] = tokens.to(self.device)[1:]
-        last = [i for i in torch.tensor([n for n in plan.q_lens if n]).cumsum(0).sub(1).tolist()]
+        last = (torch.tensor([n for n in plan.q_lens if n], dtype=torch.int64).cumsum(0) - 1).to(self.device)
         nxt[last] = -1
         parts = [scoring.token_logprobs(x[a:a + chunk] @ self.lm_head.t(), nxt[a:a + chunk], top)
                  for a in range(0, max(plan.q_tokens, 1), chunk)]

@@ -37,7 +37,7 @@ class PrefillPlan:
     ``q_lens`` / ``k_lens``: host lengths per sequence (``k_lens`` None: equal to ``q_lens``). ``rows``: the cache row of
     each sequence, for ``rebuild_kv`` (None: 0, 1, ...). Building a plan copies it to ``device`` and waits for the copy, so
     build it outside a CUDA graph capture; it can then be used on any stream of that device, by any number of calls, also
-    at the same time."""
+    at the same time. Keep it as long as a captured graph that uses it."""
 
     def __init__(self, q_lens: Sequence[int], k_lens: Optional[Sequence[int]] = None, *, n_q_heads: int, n_kv_heads: int,
                  rows: Optional[Sequence[int]] = None, device="cuda"):
@@ -74,9 +74,9 @@ class PrefillPlan:
         self._ws_bytes, self._index = {}, None
         self.host = host[:int(self.info.bytes)]
         self.data = self.host.to(self.device)
-        stream = torch.cuda.current_stream(self.device)
-        stream.synchronize()
-        self._stream = stream.cuda_stream
+        self._made_on = torch.cuda.current_stream(self.device)
+        self._made_on.synchronize()
+        self._stream = self._made_on.cuda_stream
         self.info_ptr, self.data_ptr = ctypes.byref(self.info), self.data.data_ptr()
 
     def workspace_bytes(self, d_v: int) -> int:
@@ -96,11 +96,14 @@ class PrefillPlan:
         """Per packed query token its cache row and its position ([q_tokens] int64 each, on the device; laid out once): the
         queries of a sequence stand at the last of its keys' positions."""
         if self._index is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call the plan's token_index (or run the step once) before capturing a CUDA graph with it")
             ql, kl = torch.tensor(self.q_lens), torch.tensor(self.k_lens)
             start = torch.repeat_interleave(kl - ql - (ql.cumsum(0) - ql), ql)
             host = torch.stack([torch.repeat_interleave(torch.tensor(self.rows), ql), torch.arange(self.q_tokens) + start])
-            self._index = host.to(self.device)
-            torch.cuda.current_stream(self.device).synchronize()
+            with torch.cuda.stream(self._made_on):  # as the plan's own memory: use_on knows its stream
+                self._index = host.to(self.device)
+            self._made_on.synchronize()
         return self._index[0], self._index[1]
 
     def status(self) -> int:
@@ -125,6 +128,13 @@ def _heads(t: torch.Tensor, what: str, tokens: int, heads: int, width: Optional[
     return t
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges that the tensors span meet."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+                           if t.numel() else t.data_ptr()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PrefillPlan, *, scale: Optional[float] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of a packed batch (palu_prefill_attn): q [q_tokens, n_q, 128], k [k_tokens, n_kv, 128] (both already
@@ -145,6 +155,8 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Prefil
     elif (tuple(out.shape) != (plan.q_tokens, plan.n_q_heads, d_v) or out.dtype != torch.bfloat16 or not out.is_contiguous()
           or out.device != dev):
         raise RuntimeError(f"out must be a contiguous bf16 {(plan.q_tokens, plan.n_q_heads, d_v)} tensor on {dev}")
+    elif any(_overlap(out, t) for t in (q, k, v)):
+        raise RuntimeError("out must not overlap q, k or v")
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return prefill_attn(q, k, v, plan, scale=scale, out=out)

@@ -34,7 +34,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     dtype, dev = logits.dtype, logits.device
     if not logits.is_cuda or not tokens.is_cuda:
         _lib.require_cuda(logits, tokens)
-    if logits.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float32) or logits.shape[1] < 1:
+    if logits.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float32) or not 1 <= logits.shape[1] < 2**31:
         raise RuntimeError(f"logits must be bf16 or fp32 [N, vocab], got {dtype} {tuple(logits.shape)}")
     n, vocab = logits.shape
     wide = tokens.dtype == torch.int64
