@@ -4,7 +4,7 @@
 // offset i sees the keys 0 .. i + k_len - q_len. With x_ij = scale q_i . k_j,
 //   o_i = sum_j exp(x_ij - m_i) v_j / l_i,   l_i = sum_j exp(x_ij - m_i),
 // in one pass over the keys with a running reference m_i and sum l_i (fp32); the exponentials are rounded to bf16
-// (half a step, 2^-9 relative) as the A operand of the second product, the two products accumulate in fp32.
+// (half a step, 2^-8 relative) as the A operand of the second product, the two products accumulate in fp32.
 //
 // A work item is (sequence, query tile, KV head): two chains of 128 rows, where a chain's row is one (position, query
 // head of the KV head's group) pair, positions outermost, so that the heads that share K and V share their tiles and

@@ -128,13 +128,6 @@ def _heads(t: torch.Tensor, what: str, tokens: int, heads: int, width: Optional[
     return t
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges that the tensors span meet."""
-    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
-                           if t.numel() else t.data_ptr()) for t in (a, b))
-    return a0 < b1 and b0 < a1
-
-
 def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PrefillPlan, *, scale: Optional[float] = None,
                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of a packed batch (palu_prefill_attn): q [q_tokens, n_q, 128], k [k_tokens, n_kv, 128] (both already
@@ -155,8 +148,12 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Prefil
     elif (tuple(out.shape) != (plan.q_tokens, plan.n_q_heads, d_v) or out.dtype != torch.bfloat16 or not out.is_contiguous()
           or out.device != dev):
         raise RuntimeError(f"out must be a contiguous bf16 {(plan.q_tokens, plan.n_q_heads, d_v)} tensor on {dev}")
-    elif any(_overlap(out, t) for t in (q, k, v)):
-        raise RuntimeError("out must not overlap q, k or v")
+    else:
+        at, end = out.data_ptr(), out.data_ptr() + out.nbytes
+        for t in (q, k, v):
+            (n, h, w), (s0, s1, _) = t.shape, t.stride()
+            if n and at < t.data_ptr() + 2 * ((n - 1) * s0 + (h - 1) * s1 + w) and t.data_ptr() < end:
+                raise RuntimeError("out must not overlap q, k or v")
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return prefill_attn(q, k, v, plan, scale=scale, out=out)
@@ -171,6 +168,18 @@ def prefill_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: Prefil
     return out
 
 
+def _refuse_rebuild(dev, k_latent, v_latent, u_k, u_v, cos, sin, page_table) -> None:
+    """Which of rebuild_kv's tensors is of the wrong type or on the wrong device."""
+    for t, what, dtype in ((k_latent, "k_latent", torch.bfloat16), (v_latent, "v_latent", torch.bfloat16),
+                           (u_k, "u_k", torch.bfloat16), (u_v, "u_v", torch.bfloat16), (cos, "cos", torch.float32),
+                           (sin, "sin", torch.float32), (page_table, "page_table", None)):
+        if t is not None and t.device != dev:
+            _lib.require_cuda(t)
+            raise RuntimeError(f"{what} is on {t.device}, the plan on {dev}")
+        if t is not None and dtype is not None and t.dtype != dtype:
+            raise RuntimeError(f"{what} must be {'fp32' if dtype == torch.float32 else 'bf16'}, got {t.dtype}")
+
+
 def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                plan: PrefillPlan, *, u_v: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None):
     """The packed keys and values of the plan's ``k_lens`` cached positions per sequence (palu_rebuild_kv), which
@@ -182,14 +191,12 @@ def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor
     128] bf16; cos / sin [>= longest k_len, 128] fp32 as the layer's tables. Sequence s reads cache row ``plan.rows[s]``.
     fp32 accumulation and rotation, one rounding to bf16."""
     dev, n_kv = plan.device, plan.n_kv_heads
-    for t, what, dtype in ((k_latent, "k_latent", torch.bfloat16), (v_latent, "v_latent", torch.bfloat16),
-                           (u_k, "u_k", torch.bfloat16), (u_v, "u_v", torch.bfloat16), (cos, "cos", torch.float32),
-                           (sin, "sin", torch.float32), (page_table, "page_table", None)):
-        if t is not None and t.device != dev:
-            _lib.require_cuda(t)
-            raise RuntimeError(f"{what} is on {t.device}, the plan on {dev}")
-        if t is not None and dtype is not None and t.dtype != dtype:
-            raise RuntimeError(f"{what} must be {'fp32' if dtype == torch.float32 else 'bf16'}, got {t.dtype}")
+    bf16, f32 = torch.bfloat16, torch.float32
+    if not (k_latent.dtype == bf16 and v_latent.dtype == bf16 and u_k.dtype == bf16 and (u_v is None or u_v.dtype == bf16)
+            and cos.dtype == f32 and sin.dtype == f32 and k_latent.device == dev and v_latent.device == dev
+            and u_k.device == dev and (u_v is None or u_v.device == dev) and cos.device == dev and sin.device == dev
+            and (page_table is None or page_table.device == dev)):
+        _refuse_rebuild(dev, k_latent, v_latent, u_k, u_v, cos, sin, page_table)
     ks, vs, us = k_latent.shape, v_latent.shape, u_k.shape
     if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3]:
         raise RuntimeError(f"k_latent and v_latent must be [B, n_groups, S, r] with the same leading dims, got {tuple(ks)} and "
@@ -220,7 +227,7 @@ def rebuild_kv(k_latent: torch.Tensor, v_latent: torch.Tensor, u_k: torch.Tensor
     k = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=dev)
     if u_v is not None:
         u_v = u_v.contiguous()
-        v = torch.empty(plan.k_tokens, n_kv, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+        v = torch.empty_like(k)
     else:
         v = torch.empty(plan.k_tokens, n_groups, r_v, dtype=torch.bfloat16, device=dev)
     stream = _lib.stream_handle(dev)

@@ -54,7 +54,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         ld = vocab
     tokens = tokens.contiguous()
     empty, f32 = torch.empty, torch.float32
-    lp, ent, tv = empty(n, dtype=f32, device=dev), empty(n, dtype=f32, device=dev), empty(n, top, dtype=f32, device=dev)
+    lp, tv = empty(n, dtype=f32, device=dev), empty(n, top, dtype=f32, device=dev)
+    ent = torch.empty_like(lp)
     ti = empty(n, top, dtype=torch.int64, device=dev)
     _lib.check(_lib.load().palu_token_logprobs(
         logits.data_ptr(), ld, _lib.PALU_BF16 if dtype == torch.bfloat16 else _lib.PALU_F32, n, vocab, tokens.data_ptr(), wide, top,
