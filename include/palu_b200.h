@@ -40,6 +40,9 @@
  *   palu_decode_attn_f4 / palu_append_latents_f4 / palu_quantize_latents_f4
  *                          <- the same over bfp4_b latent caches, in the B200 form: e2m1 codes with one
  *                             power-of-two scale per block of 16 values.
+ * Without a counterpart in the reference (serving): palu_plan_prefill, palu_prefill_attn, palu_rebuild_kv (packed
+ * prompts), palu_token_logprobs (scores), palu_reserve_pages, palu_fork_pages, palu_free_pages, palu_compact_pages,
+ * palu_copy_pages (pages of paged caches).
  */
 #ifndef PALU_B200_H
 #define PALU_B200_H

@@ -27,7 +27,8 @@
 // are 1024), one behind the other: 3230 a tile for both chains, against 2580 if the tensor cores never waited. Measured, 32
 // query and 8 KV heads: 32768 tokens, d_v 128 7.7 ms (1140 TFLOP/s, under the power cap); 8192 tokens 470 us (1170); d_v 64
 // 429 us (960). Tried and not kept: a polynomial for every second to eighth exponential (no faster at any share: the chain's
-// latency is what counts), S in two halves of 64 keys so that the upper one need not wait for PV (9.2 ms: an MMA takes its 64
+// latency is what counts), leaving out the keys of a diagonal tile that a chain does not see (PV alone, by predicates: 117 -> 123
+// us for 8 prompts of 64 to 2048 tokens; the exponentials too, as a second body for at most 64 keys: 120), S in two halves of 64 keys so that the upper one need not wait for PV (9.2 ms: an MMA takes its 64
 // cycles at N = 64 too).
 //
 // Masked places hold anything. Scores behind a row's last visible key are replaced, never added to. V rows behind the

@@ -11,10 +11,11 @@
 // (once per latent head; from a paged cache one box a page) and U_h, tcgen05.mma writes D = c U (128 x 128, f32) to one of
 // four TMEM buffers, and 8 warps turn it into results: a thread has a token's row and 64 head dims (a warp reads the 32 TMEM
 // lanes of its quarter), with the token's 32 frequencies of the table in registers for all heads of the unit; the rows leave
-// through shared memory by TMA (stored by the lanes, the stores took half of the warps' time: 196 us for 32 x 8192 tokens). Two warps bring the next unit's table rows to shared memory meanwhile
-// (loaded by the warps that use them, between units, they cost as much as the unit's heads). Warps 0..7: results, 8: TMA
-// producer, 9: MMA issuer, 10 and 11: table. Every wait is
-// bounded; on expiry the plan's status word is set and the unit's remaining results become NaN.
+// through shared memory by TMA. Two warps bring the next unit's table rows to shared memory meanwhile (loaded by the warps
+// that use them, between units, they cost as much as the unit's heads). 32 rows of 8192 tokens, 8 heads, rank 64: K 171 us
+// (4700 GB/s; 196 with the results stored by the lanes), with the copy of absorbed V 262. Warps 0..7: results, 8: TMA
+// producer, 9: MMA issuer, 10 and 11: table. Every wait is bounded; on expiry the plan's status word is set and the unit's
+// remaining results become NaN.
 #pragma once
 #include "prefill_tc.cuh"
 
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Absorbed V: the cached latents of a tile's tokens as they are, 8 lanes 128 bytes of a token and latent head. A copy: bound by
-// reading and writing it once.
+// reading and writing it once (32 rows of 8192 tokens, 8 latent heads of 64: 84 us, 6400 GB/s).
 constexpr int kGatherThreads = 256;
 __global__ void __launch_bounds__(kGatherThreads) palu_gather_latents_kernel(const Params p) {
   const int4 tile = p.tiles[blockIdx.x];
