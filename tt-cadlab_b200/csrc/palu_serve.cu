@@ -444,6 +444,7 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.tiles = reinterpret_cast<const int4*>(static_cast<const char*>(plan_data) + plan->off_tiles);
   p.n_kv = plan->n_kv_heads;
   p.n_groups = n_groups;
+  p.group = p.n_kv / n_groups;
   p.r_k = r_k;
   p.r_v = r_v;
   p.max_seq = max_seq;

@@ -41,7 +41,7 @@ struct Params {
   const int4* tiles;                               // row, first position, packed token, tokens (<= 128)
   const int32_t* page_table;                       // null: contiguous [B][n_groups][max_seq][r]
   int table_ld, blk_shift, n_blocks;
-  int n_kv, n_groups, r_k, r_v, max_seq;
+  int n_kv, n_groups, group, r_k, r_v, max_seq;    // group: KV heads of a latent head
   int jobs, per_unit, runs, units;                 // heads to multiply (K, then V), per unit, runs of them, units in all
   int ring, a_bytes, u_bytes, out_bufs;            // slots of the latent and the U ring, bytes of one; result buffers a warp
   int* status;
@@ -52,22 +52,44 @@ PALU_DEVINL void cp_async4(uint32_t dst, const float* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src) : "memory");
 }
 
-// A head to multiply.
-struct Job {
-  bool is_v, new_a, last_of_a;  // new_a: its latents differ from the job's before it; last_of_a: from the one's behind it
-  int h, g, r;
+// The heads of a unit, one after another: K of all heads, then V. No division in the loops over them (of a single warp's time
+// they took more than the products).
+struct Jobs {
+  int j0, j1, job, h, g, k, gs;  // k: the head's place in its group of gs
+  PALU_DEVINL Jobs(const Params& p, int run) {
+    j0 = job = run * p.per_unit;
+    j1 = min(p.jobs, j0 + p.per_unit);
+    gs = p.group;
+    h = job >= p.n_kv ? job - p.n_kv : job;
+    g = h / gs;
+    k = h - g * gs;
+  }
+  PALU_DEVINL bool more() const { return job < j1; }
+  PALU_DEVINL bool is_v(const Params& p) const { return job >= p.n_kv; }
+  PALU_DEVINL bool new_a() const { return job == j0 || k == 0; }                // its latents differ from the job's before it
+  PALU_DEVINL bool last_of_a() const { return job == j1 - 1 || k == gs - 1; }  // and from the one's behind it
+  PALU_DEVINL void next(const Params& p) {
+    ++job;
+    if (job == p.n_kv) h = g = k = 0;
+    else {
+      ++h;
+      if (++k == gs) {
+        k = 0;
+        ++g;
+      }
+    }
+  }
 };
-PALU_DEVINL Job job_of(const Params& p, int job, int j0, int j1) {
-  const int gs = p.n_kv / p.n_groups;
-  Job x;
-  x.is_v = job >= p.n_kv;
-  x.h = x.is_v ? job - p.n_kv : job;
-  x.g = x.h / gs;
-  x.r = x.is_v ? p.r_v : p.r_k;
-  x.new_a = job == j0 || x.h % gs == 0;
-  x.last_of_a = job == j1 - 1 || (x.h + 1) % gs == 0;
-  return x;
-}
+// A place in a ring of `n`, and the parity of how often it has been passed.
+struct Place {
+  int at = 0, turn = 0;
+  PALU_DEVINL void next(int n) {
+    if (++at == n) {
+      at = 0;
+      ++turn;
+    }
+  }
+};
 
 __global__ void __launch_bounds__(kThreads, 1)
     palu_rebuild_kv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -133,18 +155,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 8) {
       if (lane == 0) {
         // ============================== TMA producer ==============================
-        int na = 0, nu = 0;
+        int na = 0, nu = 0;  // copies so far
+        Place pa, pu;
         bool ok = true;
         for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-          const int4 tile = p.tiles[u / p.runs];
-          const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
-          for (int job = j0; ok && job < j1; ++job) {
-            const Job x = job_of(p, job, j0, j1);
-            if (x.new_a) {
-              const int s = na % p.ring, use = na / p.ring;
-              if (use >= 1 && !(ok = wait(bar(B_AE + s), (use - 1) & 1))) break;
-              const CUtensorMap* tm = x.is_v ? &tm_v : &tm_k;
-              const int nbox = (x.r + 63) >> 6;
+          const int t = u / p.runs;
+          const int4 tile = p.tiles[t];
+          for (Jobs x(p, u - t * p.runs); x.more(); x.next(p)) {
+            const bool is_v = x.is_v(p);
+            const int r = is_v ? p.r_v : p.r_k;
+            if (x.new_a()) {
+              const int s = pa.at;
+              if (pa.turn >= 1 && !(ok = wait(bar(B_AE + s), (pa.turn - 1) & 1))) break;
+              const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
+              const int nbox = (r + 63) >> 6;
               const uint32_t dst = sbase + s * p.a_bytes, full = bar(B_AF + s);
               mbar_expect_tx(full, nbox * kBox);
               if (!p.page_table) {
@@ -164,14 +188,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
               }
               ++na;
+              pa.next(p.ring);
             }
-            const int s = nu % p.ring, use = nu / p.ring;
-            if (use >= 1 && !(ok = wait(bar(B_UE + s), (use - 1) & 1))) break;
-            const CUtensorMap* tm = x.is_v ? &tm_uv : &tm_uk;
-            mbar_expect_tx(bar(B_UF + s), x.r * 256);
+            const int s = pu.at;
+            if (pu.turn >= 1 && !(ok = wait(bar(B_UE + s), (pu.turn - 1) & 1))) break;
+            const CUtensorMap* tm = is_v ? &tm_uv : &tm_uk;
+            mbar_expect_tx(bar(B_UF + s), r * 256);
             for (int c = 0; c < 2; ++c)
-              tma_load_2d(sbase + off_u + s * p.u_bytes + c * x.r * 128, tm, bar(B_UF + s), c * 64, x.h * x.r);
+              tma_load_2d(sbase + off_u + s * p.u_bytes + c * r * 128, tm, bar(B_UF + s), c * 64, x.h * r);
             ++nu;
+            pu.next(p.ring);
           }
         }
         if (*s_abort) {  // let every copy already issued land before the CTA can exit
@@ -183,28 +209,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 9) {
       // ============================== MMA issuer ==============================
       constexpr uint32_t ID = idesc_f16(128, 1, false, true);  // latents (K-major) x U (MN-major)
-      int na = -1, nu = 0;
+      int nu = 0;
+      Place pa, pu;
       bool ok = true;
       for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-        const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
-        for (int job = j0; job < j1; ++job) {
-          const Job x = job_of(p, job, j0, j1);
-          na += x.new_a;
-          const int sa = na % p.ring, su = nu % p.ring, d = nu % kDBufs, use = nu / kDBufs;
-          if (x.new_a && !(ok = wait_all(bar(B_AF + sa), (na / p.ring) & 1))) break;
-          if (!(ok = wait_all(bar(B_UF + su), (nu / p.ring) & 1))) break;
+        for (Jobs x(p, u % p.runs); x.more(); x.next(p)) {
+          const int r = x.is_v(p) ? p.r_v : p.r_k;
+          const int sa = pa.at, su = pu.at, d = nu % kDBufs, use = nu / kDBufs;
+          if (x.new_a() && !(ok = wait_all(bar(B_AF + sa), pa.turn & 1))) break;
+          if (!(ok = wait_all(bar(B_UF + su), pu.turn & 1))) break;
           if (use >= 1 && !(ok = wait_all(bar(B_DE + d), (use - 1) & 1))) break;
           fence_after();
-          const uint64_t a = sdesc(sbase + sa * p.a_bytes, 16, 1024), b = sdesc(sbase + off_u + su * p.u_bytes, x.r * 128, 1024);
+          const bool last = x.last_of_a();
+          const uint64_t a = sdesc(sbase + sa * p.a_bytes, 16, 1024), b = sdesc(sbase + off_u + su * p.u_bytes, r * 128, 1024);
           if (elect_one()) {
-            for (int kk = 0; kk < x.r >> 4; ++kk)
+            for (int kk = 0; kk < r >> 4; ++kk)
               mma_ss(tmem + d * 128, a + (((kk >> 2) * kBox + (kk & 3) * 32) >> 4), b + kk * (2048 >> 4), ID, kk > 0);
             mma_commit(bar(B_DF + d));
             mma_commit(bar(B_UE + su));
-            if (x.last_of_a) mma_commit(bar(B_AE + sa));
+            if (last) mma_commit(bar(B_AE + sa));
           }
           __syncwarp();
           ++nu;
+          pu.next(p.ring);
+          if (last) pa.next(p.ring);
         }
       }
       if (elect_one()) mma_commit(bar(B_DRAIN));
@@ -245,10 +273,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int nu = 0, n_t = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
-      const int4 tile = p.tiles[u / p.runs];
-      const int j0 = (u % p.runs) * p.per_unit, j1 = min(p.jobs, j0 + p.per_unit);
+      const int t = u / p.runs;
+      const int4 tile = p.tiles[t];
+      Jobs x(p, u - t * p.runs);
       float cs[32], sn[32];  // the token's frequencies 32 half .. + 31
-      if (j0 < p.n_kv) {
+      if (x.j0 < p.n_kv) {
         if (ok) ok = wait_all_inline(bar(B_TF), n_t & 1);
         ++n_t;
         const unsigned char* at = smem + off_table + row * 512 + half * 128;
@@ -268,9 +297,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_TE));
       }
-      for (int job = j0; job < j1; ++job) {
-        const Job x = job_of(p, job, j0, j1);
-        __nv_bfloat16* dst = (x.is_v ? p.v_out : p.k_out) + ((int64_t)(tile.z + quarter * 32) * p.n_kv + x.h) * kHeadDim + 64 * half;
+      for (; x.more(); x.next(p)) {
+        const bool is_v = x.is_v(p);
+        __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + ((int64_t)(tile.z + quarter * 32) * p.n_kv + x.h) * kHeadDim + 64 * half;
         const int64_t step = (int64_t)p.n_kv * kHeadDim;
         if (ok) {
           const int d = nu % kDBufs;
@@ -287,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_DE + d));
-            if (!x.is_v) {
+            if (!is_v) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
@@ -297,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             // the warp's 32 rows x 128 bytes in the layout that a swizzled TMA store takes; whole blocks of rows go out by TMA,
             // those that the tile's end cuts by the lanes
-            unsigned char* stage = smem + off_out + ((nu % p.out_bufs) * 8 + warp) * kOutBytes;
+            unsigned char* stage = smem + off_out + ((nu & (p.out_bufs - 1)) * 8 + warp) * kOutBytes;
             if (lane == 0) {
               if (p.out_bufs == 2) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
               else asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
@@ -315,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               __syncwarp();
               if (lane == 0)
                 asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(
-                                 reinterpret_cast<uint64_t>(x.is_v ? &tm_vo : &tm_ko)),
+                                 reinterpret_cast<uint64_t>(is_v ? &tm_vo : &tm_ko)),
                              "r"(smem_u32(stage)), "r"(64 * half), "r"(x.h), "r"(tile.z + quarter * 32)
                              : "memory");
             } else {
