@@ -59,7 +59,7 @@ def test_every_query_tile_is_covered_once(q_lens, k_lens, n_q, n_kv):
             assert sorted(x[2] for x in parts) == list(range(m[4], m[4] + m[5]))
     # 128-token tiles of the cached rows, for the rebuild
     at = 0
-    for t in tiles:
+    for t in sorted(tiles, key=lambda t: t[2]):
         assert t[2] == at and 0 < t[3] <= 128
         at += t[3]
     assert at == sum(k_lens)
@@ -73,7 +73,7 @@ def test_long_keys_behind_few_queries_are_split():
 
 def test_cache_rows_reach_the_rebuild_tiles():
     tiles = plan([0, 0], [140, 3], 4, 4, rows=[5, 2])[4]
-    assert tiles == [[5, 0, 0, 128], [5, 128, 128, 12], [2, 0, 140, 3]]
+    assert tiles == [[5, 0, 0, 128], [2, 0, 140, 3], [5, 128, 128, 12]]
 
 
 @pytest.mark.parametrize("args,needle", [

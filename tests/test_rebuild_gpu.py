@@ -123,3 +123,22 @@ def test_refusals(cuda):
                        ("heads_per_group", dict(k=k[:, :1].expand(-1, 3, -1, -1), v=v[:, :1].expand(-1, 3, -1, -1)))):
         with pytest.raises(RuntimeError, match=needle):
             call(**kw)
+
+
+@pytest.mark.parametrize("absorbed", [False, True])
+def test_an_expired_wait_gives_nan_and_a_status(cuda, absorbed):
+    from palu_b200 import _lib, prefill
+    lens = [200, 1, 33]
+    k, v, u_k, u_v = (x.to(cuda) if x is not None else None for x in make(lens, [0, 1, 2], 4, 1, 64, 32, absorbed))
+    cos, sin = (t.to(cuda) for t in tables(200))
+    plan = prefill.PrefillPlan([0] * 3, lens, n_q_heads=4, n_kv_heads=4, device=cuda)
+    want = prefill.rebuild_kv(k, v, u_k, cos, sin, plan, u_v=u_v)
+    _lib.set_wait_limit(2_000_000, True)                    # 2 ms; the producer loads no factors
+    try:
+        got = prefill.rebuild_kv(k, v, u_k, cos, sin, plan, u_v=u_v)
+        torch.cuda.synchronize()
+    finally:
+        _lib.set_wait_limit(0, False)
+    assert torch.isnan(got[0]).all() and (torch.equal(got[1], want[1]) if absorbed else torch.isnan(got[1]).all())
+    assert plan.status() == 1 and plan.status() == 0
+    assert all(torch.equal(a, b) for a, b in zip(prefill.rebuild_kv(k, v, u_k, cos, sin, plan, u_v=u_v), want))

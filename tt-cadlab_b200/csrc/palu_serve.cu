@@ -128,6 +128,7 @@ void make_lists(const int32_t* q_lens, const int32_t* k_lens, const int32_t* row
                 int ctas, Lists& out) {
   std::vector<Item> items;
   int32_t q0 = 0, k0 = 0;
+  size_t group = 0;
   for (int s = 0; s < n_seq; ++s) {
     const int ql = q_lens[s], kl = k_lens[s], step = 2 * ppt;
     for (int a = 0; a < ql; a += step) {
@@ -138,6 +139,10 @@ void make_lists(const int32_t* q_lens, const int32_t* k_lens, const int32_t* row
       out.tiles.push_back(make_int4(rows ? rows[s] : s, a, k0 + a, std::min(palu::rb::kTokens, kl - a)));
     q0 += ql;
     k0 += kl;
+    if (s % palu::rb::kBlock == palu::rb::kBlock - 1 || s == n_seq - 1) {  // the same positions of some sequences next to one another
+      std::stable_sort(out.tiles.begin() + group, out.tiles.end(), [](const int4& a, const int4& b) { return a.y < b.y; });
+      group = out.tiles.size();
+    }
   }
   std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.tiles > b.tiles; });
   int64_t total = 0;
@@ -450,6 +455,7 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.max_seq = max_seq;
   p.status = reinterpret_cast<int*>(const_cast<void*>(plan_data));
   p.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
+  p.starve = g_starve_v.load(std::memory_order_relaxed);
   p.jobs = u_v ? 2 * p.n_kv : p.n_kv;
   // runs of heads: as many as it takes to give every SM a unit (a unit reads its tokens' table rows once)
   const int sms = device_sms();
@@ -457,7 +463,10 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   p.per_unit = (p.jobs + runs - 1) / runs;
   p.runs = (p.jobs + p.per_unit - 1) / p.per_unit;
   if ((int64_t)plan->n_tiles * p.runs > (1 << 30)) return fail(PALU_ERR_INVALID, "rebuild: too many tiles");
-  p.units = plan->n_tiles * p.runs;
+  const int units = plan->n_tiles * p.runs, ctas = std::min(units, sms);
+  p.waves = units / (ctas * palu::rb::kBlock);
+  p.rest = (units - p.waves * ctas * palu::rb::kBlock) / ctas;
+  p.rest_more = (units - p.waves * ctas * palu::rb::kBlock) % ctas;
   const int r_max = u_v ? std::max(r_k, r_v) : r_k;
   p.a_bytes = (r_max + 63) / 64 * palu::tc::kBox;
   p.u_bytes = (r_max * 256 + 1023) / 1024 * 1024;
@@ -500,7 +509,7 @@ int palu_rebuild_kv(const void* k_lat, const void* v_lat, const void* u_k, const
   }
   static std::atomic<uint64_t> done{0};
   if (int st = allow_smem((const void*)palu::rb::palu_rebuild_kv_kernel, palu::tc::kSmemBudget, done, "cudaFuncSetAttribute(rebuild)")) return st;
-  palu::rb::palu_rebuild_kv_kernel<<<std::min(p.units, sms), palu::rb::kThreads, smem, stream>>>(mk, mv, muk, muv, mko, mvo, p);
+  palu::rb::palu_rebuild_kv_kernel<<<ctas, palu::rb::kThreads, smem, stream>>>(mk, mv, muk, muv, mko, mvo, p);
   if (int st = cuda_check("rebuild kernel launch")) return st;
   if (u_v) return PALU_OK;
   const int heads = (int)std::min<int64_t>(n_groups, std::max<int64_t>(1, 4LL * sms / plan->n_tiles));

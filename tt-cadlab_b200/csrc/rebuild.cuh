@@ -10,12 +10,15 @@
 // A unit is 128 tokens of a row and a run of heads; CTAs are persistent, one an SM. Per head: TMA brings the latents' tile
 // (once per latent head; from a paged cache one box a page) and U_h, tcgen05.mma writes D = c U (128 x 128, f32) to one of
 // four TMEM buffers, and 8 warps turn it into results: a thread has a token's row and 64 head dims (a warp reads the 32 TMEM
-// lanes of its quarter), with the token's 32 frequencies of the table in registers for all heads of the unit; the rows leave
-// through shared memory by TMA. Two warps bring the next unit's table rows to shared memory meanwhile (loaded by the warps
-// that use them, between units, they cost as much as the unit's heads). 32 rows of 8192 tokens, 8 heads, rank 64: K 171 us
-// (4700 GB/s; 196 with the results stored by the lanes), with the copy of absorbed V 262. Warps 0..7: results, 8: TMA
-// producer, 9: MMA issuer, 10 and 11: table. Every wait is bounded; on expiry the plan's status word is set and the unit's
-// remaining results become NaN.
+// lanes of its quarter), with the token's 32 frequencies of the table in registers for all heads of the unit. A warp of its
+// own sends the rows on from shared memory by TMA, so that the result warps wait for no store (each of them issuing its own
+// took 25 % of its time; stored by the lanes, half). Four warps bring the next unit's table rows to shared memory meanwhile
+// (loaded by the warps that use them, between units, they cost as much as the unit's heads); neighbouring units of the same
+// positions share them. Warps 0..7: results, 8: TMA producer, 9: MMA issuer, 10: stores, 12 to 15: table.
+//
+// 32 rows of 8192 tokens, 8 heads, rank 64: K 152 us (805 MB), with the copy of absorbed V 237. The 537 MB of results alone
+// take 139 us at the rate at which this GPU writes without reading (3850 GB/s, a plain fill); without the table's loads K takes
+// 143. Every wait is bounded; on expiry the plan's status word is set and the results not yet written become NaN.
 #pragma once
 #include "prefill_tc.cuh"
 
@@ -27,9 +30,11 @@ using palu::pf::elect_one;
 using palu::pf::touch16;
 using palu::pf::tmem_ld32p;
 
-constexpr int kTokens = 128, kThreads = 384, kDBufs = 4, kMaxRing = 4;
-constexpr int kRoleRegs = 104, kResultRegs = 200;  // of the 168 x 384 launched
-static_assert(4 * 32 * kRoleRegs + 8 * 32 * kResultRegs <= kThreads * 168, "the warpgroups' shares of the launch's registers");
+constexpr int kTokens = 128, kThreads = 512, kDBufs = 4, kMaxRing = 4, kTableWarps = 4;
+// Neighbouring units of a CTA. 32 rows of 8192 tokens, us, with 1 / 2 / 4 / 8: 259, 246, 241, 239.
+constexpr int kBlock = 4;
+constexpr int kRoleRegs = 72, kResultRegs = 184;  // of the 128 x 512 launched
+static_assert(8 * 32 * kRoleRegs + 8 * 32 * kResultRegs <= kThreads * 128, "the warpgroups' shares of the launch's registers");
 constexpr int kOutBytes = 32 * 128;          // a warp's 32 rows x 64 results
 constexpr int kTableBytes = kTokens * 512;  // a token's 64 cosines, then its 64 sines (fp32)
 constexpr int kFixedSmem = kTableBytes + 512 + 1024;  // and the rings, and one or two sets of the 8 warps' result buffers
@@ -42,10 +47,12 @@ struct Params {
   const int32_t* page_table;                       // null: contiguous [B][n_groups][max_seq][r]
   int table_ld, blk_shift, n_blocks;
   int n_kv, n_groups, group, r_k, r_v, max_seq;    // group: KV heads of a latent head
-  int jobs, per_unit, runs, units;                 // heads to multiply (K, then V), per unit, runs of them, units in all
+  int jobs, per_unit, runs;                        // heads to multiply (K, then V), per unit, runs of them
+  int waves, rest, rest_more;                      // whole rounds of kBlock units a CTA; of what is left, units a CTA, CTAs with one more
   int ring, a_bytes, u_bytes, out_bufs;            // slots of the latent and the U ring, bytes of one; result buffers a warp
   int* status;
   unsigned long long wait_ns;
+  int starve;  // test of the timeout path: the producer loads no U
 };
 
 PALU_DEVINL void cp_async4(uint32_t dst, const float* src) {
@@ -80,6 +87,44 @@ struct Jobs {
     }
   }
 };
+// A CTA's units: kBlock neighbours of every kBlock * gridDim.x, and its share of what is left over. (The plan puts the tiles
+// of the same positions of up to kBlock sequences next to one another, so neighbours share the table's rows, while the CTAs
+// together stay in a small part of the caches and results.)
+struct Walk {
+  int tile, run, left, wave;  // left: units to go in the CTA's block
+  PALU_DEVINL explicit Walk(const Params& p) {
+    wave = 0;
+    block(p);
+  }
+  PALU_DEVINL void block(const Params& p) {
+    const int c = blockIdx.x, base = wave * (int)gridDim.x * kBlock;
+    const int at = wave < p.waves ? base + c * kBlock : base + c * p.rest + min(c, p.rest_more);
+    left = wave < p.waves ? kBlock : p.rest + (c < p.rest_more);
+    tile = at / p.runs;
+    run = at - tile * p.runs;
+  }
+  PALU_DEVINL bool more() const { return left > 0; }
+  PALU_DEVINL void next(const Params& p) {
+    if (++run == p.runs) {
+      run = 0;
+      ++tile;
+    }
+    if (--left == 0 && wave < p.waves) {
+      ++wave;
+      block(p);
+    }
+  }
+};
+// Whether the table's rows of a unit's tokens are those that the CTA holds already.
+struct Held {
+  int pos = -1, tokens = 0;
+  PALU_DEVINL bool has(const int4& tile) {
+    if (tile.y == pos && tile.w <= tokens) return true;
+    pos = tile.y;
+    tokens = tile.w;
+    return false;
+  }
+};
 // A place in a ring of `n`, and the parity of how often it has been passed.
 struct Place {
   int at = 0, turn = 0;
@@ -105,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_table + kTableBytes);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   constexpr int B_AF = 0, B_AE = kMaxRing, B_UF = 2 * kMaxRing, B_UE = 3 * kMaxRing, B_DF = 4 * kMaxRing, B_DE = B_DF + kDBufs,
-                B_TF = B_DE + kDBufs, B_TE = B_TF + 1, B_DRAIN = B_TE + 1, B_COUNT = B_DRAIN + 1;
+                B_TF = B_DE + kDBufs, B_TE = B_TF + 1, B_OF = B_TE + 1, B_OE = B_OF + 2, B_DRAIN = B_OE + 2, B_COUNT = B_DRAIN + 1;
   static_assert(B_COUNT * 8 + 16 <= 512, "misc area");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
@@ -133,8 +178,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < B_DE; ++i) mbar_init(bar(i), 1);
     for (int i = 0; i < kDBufs; ++i) mbar_init(bar(B_DE + i), 8);
-    mbar_init(bar(B_TF), 2);
+    mbar_init(bar(B_TF), kTableWarps);
     mbar_init(bar(B_TE), 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(B_OF + i), 8);
+      mbar_init(bar(B_OE + i), 1);
+    }
     mbar_init(bar(B_DRAIN), 1);
     *s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
@@ -158,10 +207,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         int na = 0, nu = 0;  // copies so far
         Place pa, pu;
         bool ok = true;
-        for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-          const int t = u / p.runs;
-          const int4 tile = p.tiles[t];
-          for (Jobs x(p, u - t * p.runs); x.more(); x.next(p)) {
+        for (Walk u(p); ok && u.more(); u.next(p)) {
+          const int4 tile = p.tiles[u.tile];
+          for (Jobs x(p, u.run); x.more(); x.next(p)) {
             const bool is_v = x.is_v(p);
             const int r = is_v ? p.r_v : p.r_k;
             if (x.new_a()) {
@@ -192,6 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const int s = pu.at;
             if (pu.turn >= 1 && !(ok = wait(bar(B_UE + s), (pu.turn - 1) & 1))) break;
+            if (p.starve) continue;
             const CUtensorMap* tm = is_v ? &tm_uv : &tm_uk;
             mbar_expect_tx(bar(B_UF + s), r * 256);
             for (int c = 0; c < 2; ++c)
@@ -212,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int nu = 0;
       Place pa, pu;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-        for (Jobs x(p, u % p.runs); x.more(); x.next(p)) {
+      for (Walk u(p); ok && u.more(); u.next(p)) {
+        for (Jobs x(p, u.run); x.more(); x.next(p)) {
           const int r = x.is_v(p) ? p.r_v : p.r_k;
           const int sa = pa.at, su = pu.at, d = nu % kDBufs, use = nu / kDBufs;
           if (x.new_a() && !(ok = wait_all(bar(B_AF + sa), pa.turn & 1))) break;
@@ -238,20 +287,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (elect_one()) mma_commit(bar(B_DRAIN));
       __syncwarp();
       mbar_drain(bar(B_DRAIN), 0);
-    } else if (warp >= 10) {
+    } else if (warp == 10) {
+      // ============================== stores ==============================
+      // A head's whole blocks of 32 rows, from the result warps' buffers, by TMA; blocks that the tile's end cuts were stored
+      // by their warps. One group of stores a head.
+      int n = 0;
+      bool ok = true;
+      for (Walk u(p); u.more(); u.next(p)) {
+        const int4 tile = p.tiles[u.tile];
+        for (Jobs x(p, u.run); x.more(); x.next(p), ++n) {
+          const int b = n & (p.out_bufs - 1), use = p.out_bufs == 2 ? n >> 1 : n;
+          const bool is_v = x.is_v(p);
+          if (ok) ok = wait_all(bar(B_OF + b), use & 1);
+          if (ok) {
+            if (elect_one()) {
+              const uint64_t map = reinterpret_cast<uint64_t>(is_v ? &tm_vo : &tm_ko);
+              for (int w = 0; w < 8; ++w)
+                if ((w & 3) * 32 + 32 <= tile.w)
+                  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(map),
+                               "r"(sbase + off_out + (b * 8 + w) * kOutBytes), "r"(64 * (w >> 2)), "r"(x.h), "r"(tile.z + (w & 3) * 32)
+                               : "memory");
+              asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+              asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+              mbar_arrive(bar(B_OE + b));
+            }
+            __syncwarp();
+          } else {  // what an expired wait kept from being computed
+            __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + ((int64_t)tile.z * p.n_kv + x.h) * kHeadDim;
+            for (int i = lane; i < tile.w * kHeadDim; i += 32) dst[(int64_t)(i >> 7) * p.n_kv * kHeadDim + (i & 127)] = __float2bfloat16(NAN);
+          }
+        }
+      }
+      if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+      __syncwarp();
+    } else if (warp >= 12) {
       // ============================== table ==============================
       // The next unit's table rows, while its predecessor's heads are worked on: 4-byte copies, which leave out each
       // frequency's second place; a lane a frequency, 32 of them 128 bytes, whose 16-byte chunk k goes to k ^ (row & 7).
       const uint32_t table = sbase + off_table + (lane & 3) * 4;
+      Held held;
       int n = 0;
       bool ok = true;
-      for (int u = blockIdx.x; ok && u < p.units; u += gridDim.x) {
-        if ((u % p.runs) * p.per_unit >= p.n_kv) continue;  // V heads only
-        const int4 tile = p.tiles[u / p.runs];
+      for (Walk u(p); ok && u.more(); u.next(p)) {
+        if (u.run * p.per_unit >= p.n_kv) continue;  // V heads only
+        const int4 tile = p.tiles[u.tile];
+        if (held.has(tile)) continue;
         if (n >= 1 && !(ok = wait_all(bar(B_TE), (n - 1) & 1))) break;
         ++n;
 #pragma unroll 4
-        for (int r = warp - 10; r < kTokens; r += 2) {
+        for (int r = warp - 12; r < kTokens; r += kTableWarps) {
           const int64_t at = (int64_t)(tile.y + min(r, tile.w - 1)) * kHeadDim + 2 * lane;
           const uint32_t to = table + r * 512 + (((lane >> 2) ^ (r & 7)) << 4);
           cp_async4(to, p.cos + at);
@@ -270,15 +354,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ============================== results ==============================
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const uint32_t tD = tmem + ((uint32_t)(quarter * 32) << 16) + 64 * half;
+    float cs[32], sn[32];  // the token's frequencies 32 half .. + 31
+    Held held;
     int nu = 0, n_t = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < p.units; u += gridDim.x) {
-      const int t = u / p.runs;
-      const int4 tile = p.tiles[t];
-      Jobs x(p, u - t * p.runs);
-      float cs[32], sn[32];  // the token's frequencies 32 half .. + 31
-      if (x.j0 < p.n_kv) {
-        if (ok) ok = wait_all_inline(bar(B_TF), n_t & 1);
+    for (Walk u(p); ok && u.more(); u.next(p)) {
+      const int4 tile = p.tiles[u.tile];
+      Jobs x(p, u.run);
+      if (x.j0 < p.n_kv && !held.has(tile)) {
+        if (!(ok = wait_all_inline(bar(B_TF), n_t & 1))) break;
         ++n_t;
         const unsigned char* at = smem + off_table + row * 512 + half * 128;
 #pragma unroll
@@ -299,74 +383,54 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (; x.more(); x.next(p)) {
         const bool is_v = x.is_v(p);
-        __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + ((int64_t)(tile.z + quarter * 32) * p.n_kv + x.h) * kHeadDim + 64 * half;
-        const int64_t step = (int64_t)p.n_kv * kHeadDim;
-        if (ok) {
-          const int d = nu % kDBufs;
-          ok = wait_all_inline(bar(B_DF + d), (nu / kDBufs) & 1);
-          ++nu;
-          if (ok) {
-            fence_after();
-            uint32_t v[64];
-            tmem_ld32p(tD + d * 128, v);
-            tmem_ld32p(tD + d * 128 + 32, v + 32);
-            tmem_wait_ld();
+        const int d = nu % kDBufs, b = nu & (p.out_bufs - 1), use = p.out_bufs == 2 ? nu >> 1 : nu;
+        if (!(ok = wait_all_inline(bar(B_DF + d), (nu / kDBufs) & 1))) break;
+        fence_after();
+        uint32_t v[64];
+        tmem_ld32p(tD + d * 128, v);
+        tmem_ld32p(tD + d * 128 + 32, v + 32);
+        tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) touch16(v + 16 * i);
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_DE + d));
-            if (!is_v) {
+        for (int i = 0; i < 4; ++i) touch16(v + 16 * i);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_DE + d));
+        if (!is_v) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
-                v[2 * i] = __float_as_uint(a * cs[i] - b * sn[i]);
-                v[2 * i + 1] = __float_as_uint(b * cs[i] + a * sn[i]);
-              }
-            }
-            // the warp's 32 rows x 128 bytes in the layout that a swizzled TMA store takes; whole blocks of rows go out by TMA,
-            // those that the tile's end cuts by the lanes
-            unsigned char* stage = smem + off_out + ((nu & (p.out_bufs - 1)) * 8 + warp) * kOutBytes;
-            if (lane == 0) {
-              if (p.out_bufs == 2) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
-              else asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
-            }
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              uint32_t h[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) h[q] = pack_bf16(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]));
-              *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            }
-            if (quarter * 32 + 32 <= tile.w) {
-              fence_proxy_async();
-              __syncwarp();
-              if (lane == 0)
-                asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(
-                                 reinterpret_cast<uint64_t>(is_v ? &tm_vo : &tm_ko)),
-                             "r"(smem_u32(stage)), "r"(64 * half), "r"(x.h), "r"(tile.z + quarter * 32)
-                             : "memory");
-            } else {
-              __syncwarp();
-              const int k = lane & 7;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
-                if (quarter * 32 + r < tile.w)
-                  *reinterpret_cast<uint4*>(dst + r * step + 8 * k) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
-              }
-              __syncwarp();
-            }
-            if (lane == 0) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");  // one group a head, empty ones among them
+          for (int i = 0; i < 32; ++i) {
+            const float a = __uint_as_float(v[2 * i]), b = __uint_as_float(v[2 * i + 1]);
+            v[2 * i] = __float_as_uint(a * cs[i] - b * sn[i]);
+            v[2 * i + 1] = __float_as_uint(b * cs[i] + a * sn[i]);
           }
         }
-        if (!ok && row < tile.w)
-          for (int i = 0; i < 64; ++i) dst[lane * step + i] = __float2bfloat16(NAN);
+        // the warp's 32 rows x 128 bytes, in the layout that a swizzled TMA store takes
+        if (use >= 1 && !(ok = wait_all_inline(bar(B_OE + b), (use - 1) & 1))) break;
+        unsigned char* stage = smem + off_out + (b * 8 + warp) * kOutBytes;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t h[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) h[q] = pack_bf16(__uint_as_float(v[8 * i + 2 * q]), __uint_as_float(v[8 * i + 2 * q + 1]));
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (quarter * 32 + 32 > tile.w) {
+          __nv_bfloat16* dst = (is_v ? p.v_out : p.k_out) + ((int64_t)(tile.z + quarter * 32) * p.n_kv + x.h) * kHeadDim + 64 * half;
+          const int64_t step = (int64_t)p.n_kv * kHeadDim;
+          const int k = lane & 7;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + (lane >> 3);
+            if (quarter * 32 + r < tile.w)
+              *reinterpret_cast<uint4*>(dst + r * step + 8 * k) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
+          }
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(bar(B_OF + b));
+        ++nu;
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
-    __syncwarp();
   }
   // every role reaches this point warp-converged
   fence_before();
