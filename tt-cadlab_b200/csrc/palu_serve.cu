@@ -3,6 +3,8 @@
 #include <algorithm>
 #include <atomic>
 #include <exception>
+#include <functional>
+#include <utility>
 #include <vector>
 
 #include "../../include/palu_b200.h"
@@ -50,16 +52,19 @@ struct Lists {
   int slots = 0;
 };
 
-// Whole items, heaviest first, dealt to the CTAs in alternating direction. Returns the largest CTA's cost.
+// Whole items, heaviest first, each to the CTA with the least so far. Returns the largest CTA's cost.
 int64_t deal_whole(const std::vector<Item>& items, int n_kv, int ctas, Lists* out) {
-  std::vector<int64_t> load(ctas, 0);
+  typedef std::pair<int64_t, int> Load;
+  std::vector<Load> heap(ctas);  // the least on top
+  for (int c = 0; c < ctas; ++c) heap[c] = {0, c};
   std::vector<std::vector<palu::pf::PfPiece>> per(out ? ctas : 0);
-  int64_t n = 0;
+  int64_t most = 0;
   for (const Item& it : items)
-    for (int h = 0; h < n_kv; ++h, ++n) {
-      const int64_t round = n / ctas, x = n % ctas;
-      const int c = (int)(round & 1 ? ctas - 1 - x : x);
-      load[c] += it.tiles + kPieceTiles;
+    for (int h = 0; h < n_kv; ++h) {
+      std::pop_heap(heap.begin(), heap.end(), std::greater<Load>());
+      const int c = heap.back().second;
+      most = std::max(most, heap.back().first += it.tiles + kPieceTiles);
+      std::push_heap(heap.begin(), heap.end(), std::greater<Load>());
       if (out) per[c].push_back({it.q0, it.npos, it.vis0, it.k0, h, 0, it.tiles, -1});
     }
   if (out) {
@@ -69,7 +74,7 @@ int64_t deal_whole(const std::vector<Item>& items, int n_kv, int ctas, Lists* ou
       out->start.push_back((int32_t)out->pieces.size());
     }
   }
-  return load.empty() ? 0 : *std::max_element(load.begin(), load.end());
+  return most;
 }
 
 // Items cut along the keys so that no CTA gets more than `share`; false if that takes more than `ctas` CTAs.
