@@ -135,5 +135,7 @@ def test_cpu_tensors_are_refused():
 def test_limits_of_the_largest_calls():
     with pytest.raises(RuntimeError, match="work items"):
         plan([1 << 28], [1], 1024, 8)                     # 2^27 query tiles x 8 KV heads
+    with pytest.raises(RuntimeError, match="65536 query heads"):
+        plan([1], [1], 1 << 17, 1 << 17)
     st, msg = _call(plan([4], [4], 4, 1)[0], scale=3e38)  # finite, but not times log2 e
     assert st == _lib.PALU_ERR_INVALID and "scale" in msg

@@ -278,6 +278,7 @@ int palu_plan_prefill(const int32_t* q_lens, const int32_t* k_lens, const int32_
   if (n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0)
     return fail(PALU_ERR_INVALID, "KV head count %d must divide the %d query heads", n_kv_heads, n_q_heads);
   const int rep = n_q_heads / n_kv_heads;
+  if (n_q_heads > 65536) return fail(PALU_ERR_INVALID, "at most 65536 query heads are supported, got %d", n_q_heads);
   if (rep > palu::pf::kRows) return fail(PALU_ERR_INVALID, "at most 128 query heads per KV head are supported, got %d", rep);
   if (n_ctas < 0 || n_ctas > 4096) return fail(PALU_ERR_INVALID, "n_ctas must be in [0, 4096], got %d", n_ctas);
   int64_t tq = 0, tk = 0, items = 0;

@@ -26,7 +26,8 @@
 // being what shared memory delivers in 512) and the softmax warps 1870 (128 exponentials of the special-function unit a row
 // are 1024), one behind the other: 3230 a tile for both chains, against 2580 if the tensor cores never waited. Measured, 32
 // query and 8 KV heads: 32768 tokens, d_v 128 7.7 ms (1140 TFLOP/s, under the power cap); 8192 tokens 470 us (1170); d_v 64
-// 429 us (960). Tried and not kept: a polynomial for every second to eighth exponential (no faster at any share: the chain's
+// 429 us (960). A piece takes about 7000 cycles besides its tiles (first reference, the last PV, an epilogue of 4000): 32
+// prompts of 512 tokens 135 us, 8 prompts of 64 to 2048 tokens 111. Tried and not kept: a polynomial for every second to eighth exponential (no faster at any share: the chain's
 // latency is what counts), leaving out the keys of a diagonal tile that a chain does not see (PV alone, by predicates: 117 -> 123
 // us for 8 prompts of 64 to 2048 tokens; the exponentials too, as a second body for at most 64 keys: 120), S in two halves of 64 keys so that the upper one need not wait for PV (9.2 ms: an MMA takes its 64
 // cycles at N = 64 too).
@@ -98,7 +99,7 @@ struct PfLayout {
   static constexpr int OFF_V = OFF_K + NS_K * kKBytes;
   static constexpr int OFF_OUT = OFF_V + NS_V * V_BYTES;  // 32 rows x 64 results (bf16) a softmax warp
   static constexpr int OFF_MISC = OFF_OUT + 8 * kOutBytes;
-  static constexpr int TOTAL = OFF_MISC + 512 + kRows * 4 + 1024;
+  static constexpr int TOTAL = OFF_MISC + 512 + kRows * 8 + 1024;
   // TMEM columns
   static constexpr uint32_t S = 0;                       // + 128 c
   static constexpr uint32_t P = ALIAS ? 0 : 256;         // + P_STEP c
@@ -187,6 +188,17 @@ PALU_DEVINL uint32_t finite_bf16x2(uint32_t w) {
   const uint32_t f = nonfinite_bf16x2(w);
   return w & ~((f >> 15 & 1u) * 0xFFFFu | (f >> 31) * 0xFFFF0000u);
 }
+// Shared memory by its own address space: loads through generic pointers stay behind the global stores before them.
+PALU_DEVINL uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+PALU_DEVINL int2 lds64(uint32_t at) {
+  int2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
 PALU_DEVINL bool elect_one() {
   uint32_t ok;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(ok));
@@ -209,15 +221,15 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Lay::OFF_MISC);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   // QF / QE: Q of chain c landed / free. KF / KE, VF / VE: ring slots. VC: the V tile of a cut tile has landed and is to
-  // be checked (by count of cut tiles, four in turn: more than the V ring holds); the checkers' two arrivals, instead of
-  // the copy's own, then complete VF, so a checker that looks at some tiles only never loses count of a phase. SF: S_c written. SR: S_c read (P of its own only). PF: P_c written. OD: PV_c done.
-  // OE: O_c read by the epilogue.
+  // be checked (by count of cut tiles, four in turn: more than the V ring holds); the arrivals of the two warps
+  // that check, instead of the copy's own, then complete VF, so that looking at some tiles only they never lose count of a
+  // phase. SF: S_c written. SR: S_c read (P of its own only). PF: P_c written. OD: PV_c done. OE: O_c read by the epilogue.
   constexpr int B_QF = 0, B_QE = 2, B_KF = 4, B_KE = B_KF + NS_K, B_VF = B_KE + NS_K, B_VE = B_VF + NS_V,
                 B_VC = B_VE + NS_V, B_SF = B_VC + 4, B_SR = B_SF + 2, B_PF = B_SR + 2, B_OD = B_PF + 2, B_OE = B_OD + 2,
                 B_DRAIN = B_OE + 2, B_COUNT = B_DRAIN + 1;
   static_assert(B_COUNT * 8 + 64 <= 512, "misc area");
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
-  int* s_row = reinterpret_cast<int*>(smem + Lay::OFF_MISC + 512);  // [128] a row's position << 8 | query head
+  int2* s_row = reinterpret_cast<int2*>(smem + Lay::OFF_MISC + 512);  // [128] a row's position and its place in the output behind the chain's
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
   volatile int* s_bad = reinterpret_cast<volatile int*>(s_tmem + 2);  // [4]: 1 + index of the last piece with non-finite V
 
@@ -268,7 +280,10 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (threadIdx.x < kRows) s_row[threadIdx.x] = (threadIdx.x / p.rep) << 8 | (threadIdx.x % p.rep);
+  if (threadIdx.x < kRows) {
+    const int pos = threadIdx.x / p.rep;
+    s_row[threadIdx.x] = make_int2(pos, (pos * p.n_q + (int)threadIdx.x - pos * p.rep) * p.dv);
+  }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
                  "r"(kTmemCols)
@@ -640,7 +655,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
       const float inv = lost ? NAN : 1.f / l;
       for (int x = 0; x < p.dv; x += 64) {
-        unsigned char* stage = smem + Lay::OFF_OUT + warp * kOutBytes;
+        const uint32_t stage = sbase + Lay::OFF_OUT + warp * kOutBytes;
         const int width = min(64, p.dv - x);
 #pragma unroll 1
         for (int y = 0; y < width; y += 32) {  // the last 16 columns may be behind d_v: read and dropped
@@ -680,26 +695,36 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               if (y + z < width) po[z * kRows] = __uint_as_float(o[z]);
           } else {
             // through shared memory, so that 8 lanes write 128 bytes of a row: chunk k of row r at chunk k ^ r & 7 (straight from
-            // the registers, every store touched 32 lines: 3000 to 4000 cycles a piece at d_v 128)
+            // the registers, every store touched 32 lines: 3000 to 4000 cycles a piece at d_v 128; now 1300, the warps' stores
+            // coming behind their loads, not in turn with them)
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
               uint32_t h[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q)
                 h[q] = vis <= 0 ? 0u : pack_bf16(__uint_as_float(o[8 * z + 2 * q]) * inv, __uint_as_float(o[8 * z + 2 * q + 1]) * inv);
-              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((y >> 3) + z) ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(smem + Lay::OFF_OUT + warp * kOutBytes + lane * 128 + ((((y >> 3) + z) ^ (lane & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
             }
           }
         }
         if (w.slot < 0) {
           __syncwarp();
-          const int k = lane & 7;
+          const int k = lane & 7, npos = min(p.ppt, w.npos - c * p.ppt);
+          __nv_bfloat16* out = p.out + (((size_t)w.q0 + c * p.ppt) * p.n_q + w.kvh * p.rep) * p.dv + x + 8 * k;
+          const uint32_t rows = sbase + Lay::OFF_MISC + 512 + ((warp & 3) * 32 + (lane >> 3)) * 8;
+#pragma unroll 1
+          for (int z0 = 0; z0 < 8; z0 += 4) {
+            uint4 v[4];
+            int2 at[4];
 #pragma unroll
-          for (int z = 0; z < 8; ++z) {
-            const int r = 4 * z + (lane >> 3), at = s_row[(warp & 3) * 32 + r], lp = c * p.ppt + (at >> 8);
-            if ((at >> 8) < p.ppt && lp < w.npos && 8 * k < width)
-              *reinterpret_cast<uint4*>(p.out + (((size_t)w.q0 + lp) * p.n_q + w.kvh * p.rep + (at & 255)) * p.dv + x + 8 * k) =
-                  *reinterpret_cast<const uint4*>(stage + r * 128 + ((k ^ (r & 7)) << 4));
+            for (int z = 0; z < 4; ++z) {
+              const int r = 4 * (z0 + z) + (lane >> 3);
+              v[z] = lds128(stage + r * 128 + ((k ^ (r & 7)) << 4));
+              at[z] = lds64(rows + (z0 + z) * 32);
+            }
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+              if (at[z].x < npos && 8 * k < width) *reinterpret_cast<uint4*>(out + at[z].y) = v[z];
           }
           __syncwarp();
         }
