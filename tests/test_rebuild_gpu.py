@@ -142,3 +142,20 @@ def test_an_expired_wait_gives_nan_and_a_status(cuda, absorbed):
     assert torch.isnan(got[0]).all() and (torch.equal(got[1], want[1]) if absorbed else torch.isnan(got[1]).all())
     assert plan.status() == 1 and plan.status() == 0
     assert all(torch.equal(a, b) for a, b in zip(prefill.rebuild_kv(k, v, u_k, cos, sin, plan, u_v=u_v), want))
+
+
+@pytest.mark.parametrize("n,n_kv,absorbed", [(400, 2, False), (400, 1, True), (70, 8, True)])
+def test_many_units_on_a_thread_block(cuda, n, n_kv, absorbed):
+    """Several units one after another on every thread block, neighbours of the same positions among them, whose tokens are
+    fewer or more than the unit's before."""
+    from palu_b200 import prefill
+    lens = [(1, 130, 64, 257, 128, 5, 300, 77, 200)[(4 * i + i // 5) % 9] for i in range(n)]
+    rows = torch.randperm(n, generator=torch.Generator().manual_seed(3)).tolist()
+    k, v, u_k, u_v = make(lens, rows, n_kv, 1, 16, 16, absorbed)
+    cos, sin = tables(300)
+    plan = prefill.PrefillPlan([0] * n, lens, n_q_heads=n_kv, n_kv_heads=n_kv, rows=rows, device=cuda)
+    gk, gv = prefill.rebuild_kv(k.to(cuda), v.to(cuda), u_k.to(cuda), cos.to(cuda), sin.to(cuda), plan,
+                                u_v=None if u_v is None else u_v.to(cuda))
+    torch.cuda.synchronize()
+    assert plan.status() == 0
+    check(gk, gv, k, v, u_k, u_v, lens, rows, cos, sin, 1)

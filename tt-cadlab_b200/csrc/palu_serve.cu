@@ -1,5 +1,5 @@
-// C ABI of the operators around the decode step: the plan and attention of packed prompts. Validation, planning and
-// dispatch on the host; the kernels live in the .cuh files next to it.
+// C ABI of the operators around the decode step: packed prompts (plan, attention, rebuilt keys and values), scores of tokens,
+// pages. Validation, planning and dispatch on the host; the kernels live in the .cuh files next to it.
 #include <algorithm>
 #include <atomic>
 #include <exception>
