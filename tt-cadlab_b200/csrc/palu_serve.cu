@@ -406,10 +406,8 @@ int palu_prefill_attn(const void* q, int64_t q_tok, int64_t q_head, const void* 
   if (plan->n_merges > 0) {
     const auto* merges = reinterpret_cast<const palu::pf::PfMerge*>(data + plan->off_merges);
     if (plan->n_slots >= palu::pf::kDeepRecords * plan->n_merges)
-      palu::pf::palu_prefill_merge_deep_kernel<<<dim3(plan->n_merges, 8, (d_v + 31) / 32), 256, 0, stream>>>(merges, p);
-    else
-      palu::pf::palu_prefill_merge_kernel<<<dim3(plan->n_merges, 8), 256, 0, stream>>>(merges, p);
-    return cuda_check("prefill merge launch");
+      return launch_dependent("prefill merge launch", palu::pf::palu_prefill_merge_deep_kernel, dim3(plan->n_merges, 8, (d_v + 31) / 32), 256, stream, merges, p);
+    return launch_dependent("prefill merge launch", palu::pf::palu_prefill_merge_kernel, dim3(plan->n_merges, 8), 256, stream, merges, p);
   }
   return PALU_OK;
 }

@@ -257,6 +257,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     return __all_sync(0xffffffffu, done) != 0;
   };
 
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the merge, which waits for this grid's end
   if (threadIdx.x == 0) {
     for (int c = 0; c < 2; ++c) {
       mbar_init(bar(B_QF + c), 1);
@@ -761,10 +762,12 @@ __global__ void __launch_bounds__(kPfThreads, 1)
 
 // Joins the records of the items that were cut along the keys: with w_s = 2^(m_s - max m),
 // o = sum_s w_s O_s / sum_s w_s l_s. A block joins 32 rows (a lane a row, a warp every eighth column) and writes them
-// through shared memory. For few records an item, whose loads it issues record by record.
+// through shared memory. For few records an item, whose loads it issues record by record. Launched as a programmatic
+// dependent of the attention (one query on 4000 keys 24.9 -> 22.4 us one call after another).
 __global__ void __launch_bounds__(256) palu_prefill_merge_kernel(const PfMerge* merges, const PfParams p) {
   __shared__ float s_o[32][129];
   const PfMerge w = merges[blockIdx.x];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = blockIdx.y * 32 + lane, c = r >> 7, row = r & 127, lpos = c * p.ppt + row / p.rep;
   if (c * p.ppt + (blockIdx.y * 32 & 127) / p.rep >= w.npos) return;  // the block's first row is behind the item
@@ -810,6 +813,7 @@ constexpr int kDeepRecords = 8;
 __global__ void __launch_bounds__(256) palu_prefill_merge_deep_kernel(const PfMerge* merges, const PfParams p) {
   __shared__ float s_o[8][32][33], s_l[8][32];
   const PfMerge w = merges[blockIdx.x];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = (int)blockIdx.y >> 2, row0 = (int)(blockIdx.y & 3) * 32, row = row0 + lane, x0 = blockIdx.z * 32;
   if (c * p.ppt + row0 / p.rep >= w.npos) return;  // the block's first row is behind the item
