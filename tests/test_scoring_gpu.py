@@ -214,3 +214,22 @@ def test_a_vocabulary_past_32_bits_is_refused(cuda):
     logits = torch.zeros(1, 1, dtype=torch.bfloat16, device=cuda).expand(1, 2**31)
     with pytest.raises(RuntimeError, match="vocab"):
         scoring.token_logprobs(logits, torch.zeros(1, dtype=torch.long, device=cuda))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [4000, 40000])
+@pytest.mark.parametrize("base", [-16000.0, -16512.0, -30080.0, -65280.0, -100352.0, -499712.0, 30080.0, 499712.0], ids=str)
+def test_rows_far_from_zero(cuda, dtype, vocab, base):
+    """Rows where a step of bf16 is 64 to 2048: every argument of an exponential is one fma against a reference, off by 2^-24
+    of the difference and not of the logits, so the tolerance stays. Low values first and the next higher step later, in
+    every part of the row that a thread block may read (from 5000 elements on); both steps mixed; one value; one higher one."""
+    g = torch.Generator().manual_seed(7)
+    step = 2.0 ** (math.floor(math.log2(abs(base))) - 7)
+    logits = torch.full((5, vocab), base)
+    logits[0, torch.arange(vocab) % 5000 >= 3500] = base + step
+    logits[1] += step / 2 + 3 * torch.randn(vocab, generator=g)
+    logits[3, vocab - 1] = base + step
+    logits[4] += 40 * torch.randn(vocab, generator=g)
+    logits = logits.to(cuda, dtype)
+    assert logits[0].unique().numel() == 2 and logits[1].unique().numel() >= 2
+    check(cuda, logits, torch.tensor([3999, 1, 2, vocab - 1, 17], device=cuda), 5)

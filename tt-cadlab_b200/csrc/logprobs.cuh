@@ -322,8 +322,10 @@ struct Run<__nv_bfloat16> {
     if (max2(m, limit) != limit || limit == kNone) {
       const float hi = max();
       if (hi > s.ref + kOutgrown) s.raise(hi);
-      // rounded towards zero: for a negative limit that is up, by less than the 2^-7 of it that the sums have room for
-      const uint32_t l = s.large() ? kNone & 0xFFFFu : __float_as_uint(s.ref + kOutgrown) >> 16;
+      // rounded down (a step of bf16 is up to 2048 here, and the sums have no room for an element that far above the
+      // reference); never below the reference, which is a bf16 value itself, so equal elements stay off this path
+      const uint32_t f = __float_as_uint(s.ref + kOutgrown);
+      const uint32_t l = s.large() ? kNone & 0xFFFFu : (f >> 16) + ((f >> 31) & ((f & 0xFFFFu) != 0));
       limit = l << 16 | l;
       if (s.large()) {
 #pragma unroll
