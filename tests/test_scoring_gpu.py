@@ -233,3 +233,21 @@ def test_rows_far_from_zero(cuda, dtype, vocab, base):
     logits = logits.to(cuda, dtype)
     assert logits[0].unique().numel() == 2 and logits[1].unique().numel() >= 2
     check(cuda, logits, torch.tensor([3999, 1, 2, vocab - 1, 17], device=cuda), 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("top", [1, 3, 32])
+@pytest.mark.parametrize("n,vocab", [(6, 3000), (7, 128256), (330, 9001)])
+def test_a_nan_anywhere_comes_first(cuda, dtype, top, n, vocab):
+    """NaN at the row's first and last places and between them, alone, twice and in numbers, of either sign, with one and with
+    eight thread blocks a row: the lowest of their ids come first, then the other logits in order."""
+    logits = torch.randn(n, vocab, generator=torch.Generator().manual_seed(vocab + top)) * 3
+    places = ([10], [vocab // 2], [vocab - 1], [0, vocab - 2], list(range(5, vocab, 61)), [])
+    for i in range(n):
+        logits[i, places[i % 6]] = math.nan if i % 4 < 2 else -math.nan
+    lp, ent, tv, ti = run(cuda, logits.to(cuda, dtype), torch.full((n,), 3, device=cuda), top)
+    bad = torch.tensor([bool(places[i % 6]) for i in range(n)])
+    want = torch.sort(logits.to(dtype).double(), dim=-1, descending=True, stable=True).indices[:, :top]   # NaN is the largest
+    assert (ti >= 0).all() and (ti < vocab).all() and torch.equal(ti, want)
+    for t in (lp, ent, tv[:, 0]):
+        assert torch.equal(torch.isnan(t), bad)

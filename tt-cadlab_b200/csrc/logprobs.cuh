@@ -355,7 +355,8 @@ struct Run<__nv_bfloat16> {
   static constexpr uint32_t kLowest2 = 0xF14AF14Au;  // -1e30 rounded to bf16, twice
 };
 
-// Where a thread's largest element is: the stage that brought it, and the largest element of the other stages.
+// Where a thread's largest element is: the stage that brought it, and the largest element of the other stages. Of no use to a
+// thread that saw a NaN (a later stage takes its place).
 struct Where {
   float best, rest;
   int stage;
@@ -365,7 +366,7 @@ struct Where {
   }
   PALU_DEVINL void add(float top, int at) {
     rest = fmaxf(rest, fminf(top, best));
-    if (!(top <= best)) {  // a NaN too; a thread that saw one has all its elements looked at
+    if (!(top <= best)) {
       best = top;
       stage = at;
     }
@@ -575,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) palu_token_logprobs_kernel(co
       };
       if (own != 0 && own >= least) {
         if (n > tid) {  // it has a chunk
-          if (order_of(where.rest) >= least || isnan(where.best)) {
+          if (order_of(where.rest) >= least || own == 0xFFFFFFFFu) {  // or a NaN among them
             s_who[atomicAdd(&s_owners, 1)] = tid;
           } else {
 #pragma unroll
