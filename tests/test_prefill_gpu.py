@@ -265,3 +265,32 @@ def test_token_index_is_not_laid_out_in_a_capture(cuda):
         torch.zeros(1, device=cuda)
         with pytest.raises(RuntimeError, match="before capturing"):
             plan.token_index()
+
+
+@pytest.mark.parametrize("d_v", [64, 128])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_a_reference_that_moves_among_large_scores(cuda, d_v, sign):
+    """Scores of about +-2^20 that are exact integers (their tolerance is that of small ones: only differences matter). Eight
+    tiles whose maxima stay within reach of the first reference, then a score that moves it: both parts weigh about the same,
+    and an error of their relative weight by x would move the result by x / 2. The offset is the one at which the two references'
+    products with log2 e, rounded to fp32, differ most."""
+    import numpy as np
+    log2e = np.float32(math.log2(math.e))
+    slip = lambda m: float(np.float32(m) * log2e) - float(m) * float(log2e)
+    base = int(sign) * 2**20
+    e = max(range(200), key=lambda e: abs(slip(base + e) - slip(base + e + 13)))
+    assert abs(slip(base + e) - slip(base + e + 13)) > 2.0 ** -4           # a weight off by 4 % if it entered the result
+    n, rows = 9 * 128, 2
+    offset = torch.full((n,), 6.0)
+    offset[:32] = 0
+    offset[1024:] = 0
+    offset[1024] = 13
+    q = torch.zeros(rows, 4, H)
+    q[..., 0], q[..., 1] = 1024 * sign, 1.0
+    k = torch.zeros(n, 1, H)
+    k[..., 0], k[..., 1] = 1024.0, (offset + e)[:, None]
+    v = torch.ones(n, 1, d_v)
+    v[1024:] = -1
+    q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
+    assert float((offset + e).max()) <= 256                                 # integers that bf16 holds
+    check(attend(cuda, q, k, v, [rows], [n], scale=1.0), q, k, v, [rows], [n], scale=1.0)

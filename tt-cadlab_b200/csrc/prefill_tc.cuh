@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
         // P of the tile against m_ref, and its sum
         auto stream = [&](auto is_cut) {
           constexpr bool CUT = decltype(is_cut)::value;
-          const float mb = m_ref == -INFINITY ? 0.f : -m_ref * p.sl2;
+          const float mb = m_ref == -INFINITY ? 0.f : -__fmul_rn(m_ref, p.sl2);
           const uint64_t sl2 = pack2(p.sl2, p.sl2), mb2 = pack2(mb, mb);
           uint64_t l2[2] = {0, 0};
           uint32_t s[2][32];
@@ -610,8 +610,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
             if (tm > m_ref && tm < INFINITY) ref = tm;
           }
           if (!__any_sync(0xffffffffu, ref != m_ref)) break;
-          // new references: O and l follow, and the tile is done over
-          const float alpha = ref == m_ref ? 1.f : (m_ref == -INFINITY ? 0.f : fast_exp2((m_ref - ref) * p.sl2));
+          // New references: O and l follow, and the tile is done over. By the references' products as the exponentials took them,
+          // each rounded: at scores of 2^20 the difference taken first is off by up to 2^-3 from theirs.
+          const float alpha = ref == m_ref ? 1.f : (m_ref == -INFINITY ? 0.f : fast_exp2(__fmul_rn(m_ref, p.sl2) - __fmul_rn(ref, p.sl2)));
           if (j > 0) {
             if (!ALIAS && !(ok = wait_all_inline(bar(B_OD + c), (n_s - 1) & 1))) break;  // PV of the tile before is in O
             fence_after();
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       if (w.slot >= 0 && have) {
         float* ml = p.ws_ml + ((size_t)w.slot * 2 * kRows + c * kRows + row) * 2;
-        ml[0] = lost ? NAN : (m_ref == -INFINITY ? -INFINITY : m_ref * p.sl2);
+        ml[0] = lost ? NAN : (m_ref == -INFINITY ? -INFINITY : __fmul_rn(m_ref, p.sl2));
         ml[1] = l;
       }
     }
