@@ -294,3 +294,40 @@ def test_a_reference_that_moves_among_large_scores(cuda, d_v, sign):
     q, k, v = (t.to(torch.bfloat16) for t in (q, k, v))
     assert float((offset + e).max()) <= 256                                 # integers that bf16 holds
     check(attend(cuda, q, k, v, [rows], [n], scale=1.0), q, k, v, [rows], [n], scale=1.0)
+
+
+def _many_short(n):
+    g = torch.Generator().manual_seed(20)
+    q = torch.randint(1, 41, (n,), generator=g).tolist()
+    return q, [x + (37 if i % 7 == 3 else 0) for i, x in enumerate(q)]
+
+
+@pytest.mark.parametrize("d_v", [48, 64, 80, 128])
+@pytest.mark.parametrize("batch", ["whole", "few_records", "many_records", "many_short"])
+def test_non_finite_values_in_every_layout_of_the_work(cuda, d_v, batch):
+    """Infinities and NaNs among the values, in the first and the last column: items that are whole, cut along the keys into
+    few and into many records, and some hundreds of short prompts one after another on a thread block. A query that sees such
+    a value gets it (of both signs, or a NaN: NaN), every other result keeps its bits."""
+    from palu_b200 import prefill
+    q_lens, k_lens = {"whole": ([90, 5, 300], [90, 5, 300]), "few_records": ([512], [2000]), "many_records": ([20], [6000]),
+                      "many_short": _many_short(700)}[batch]
+    plan = prefill.PrefillPlan(q_lens, k_lens, n_q_heads=8, n_kv_heads=2, device=cuda).info
+    assert {"few_records": 0 < plan.n_merges * 2 <= plan.n_slots < 8 * plan.n_merges, "many_records": 0 < 8 * plan.n_merges <= plan.n_slots,
+            "many_short": plan.n_merges == 0 and plan.n_pieces >= 4 * plan.n_ctas}.get(batch, plan.n_merges == 0)
+    q, k, v = inputs(q_lens, k_lens, 8, 2, d_v, seed=21)
+    bad, q0, k0 = [], 0, 0                                    # (first query row, its end, key row, KV head, column, value)
+    for s, (ql, kl) in enumerate(zip(q_lens, k_lens)):
+        if batch != "many_short" or s % 5 == 0:
+            for i, h, x, y in ((ql // 3, 0, 0, math.inf), (ql // 2, 0, 0, -math.inf), (ql // 2, 1, d_v - 1, math.nan),
+                               (ql - 1, 0, d_v - 1, math.inf)):
+                bad.append((q0 + i, q0 + ql, k0 + kl - ql + i, h, x, y))
+        q0, k0 = q0 + ql, k0 + kl
+    v2 = v.clone()
+    for b in bad:
+        v2[b[2], b[3], b[4]] = b[5]
+    clean = attend(cuda, q, k, v, q_lens, k_lens).float().cpu()
+    got = attend(cuda, q, k, v2, q_lens, k_lens).float().cpu()
+    want = clean.clone()
+    for b in bad:
+        want[b[0]:b[1], 4 * b[3]:4 * b[3] + 4, b[4]] += v2[b[2], b[3], b[4]].float()
+    assert torch.equal(torch.nan_to_num(got, nan=7e30, posinf=8e30, neginf=9e30), torch.nan_to_num(want, nan=7e30, posinf=8e30, neginf=9e30))

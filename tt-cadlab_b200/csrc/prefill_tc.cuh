@@ -232,7 +232,9 @@ __global__ void __launch_bounds__(kPfThreads, 1)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   int2* s_row = reinterpret_cast<int2*>(smem + Lay::OFF_MISC + 512);  // [128] a row's position and its place in the output behind the chain's
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  volatile int* s_bad = reinterpret_cast<volatile int*>(s_tmem + 2);  // [4]: 1 + index of the last piece with non-finite V
+  // 1 + index of the last piece with non-finite V so far. It only grows, so an epilogue that comes late still sees its piece's
+  // mark; a mark of a later piece makes it look at V rows that hold nothing to add.
+  volatile int* s_bad = reinterpret_cast<volatile int*>(s_tmem + 2);
 
   auto wait = [&](uint32_t b, uint32_t ph) -> bool { return mbar_wait(b, ph, s_abort, p.status, p.wait_ns); };
   auto wait_all = [&](uint32_t b, uint32_t ph) -> bool {
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
     for (int s = 0; s < 4; ++s) mbar_init(bar(B_VC + s), 1);
     mbar_init(bar(B_DRAIN), 1);
     *s_abort = 0;
-    s_bad[0] = s_bad[1] = s_bad[2] = s_bad[3] = 0;
+    *s_bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   if (threadIdx.x < kRows) {
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
               }
             }
           }
-          if (bad) s_bad[i & 3] = i + 1;
+          if (bad) atomicMax(const_cast<int*>(s_bad), i + 1);
           fence_proxy_async();  // these reads and writes before the tensor core's reads and the slot's next copy
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(B_VF + sv));
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(kPfThreads, 1)
       }
       // a NaN or +infinity among the row's scores makes the row NaN, as do scores that are all -infinity
       const bool lost = isnan(m_true) || m_true == INFINITY || (m_ref == -INFINITY && vis > 0 && w.slot < 0);
-      const bool bad = nt > 0 && s_bad[i & 3] == i + 1;
+      const bool bad = nt > 0 && *s_bad > i;
       const float inv = lost ? NAN : 1.f / l;
       for (int x = 0; x < p.dv; x += 64) {
         const uint32_t stage = sbase + Lay::OFF_OUT + warp * kOutBytes;
