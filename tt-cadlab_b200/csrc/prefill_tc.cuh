@@ -26,8 +26,8 @@
 // being what shared memory delivers in 512) and the softmax warps 1870 (128 exponentials of the special-function unit a row
 // are 1024), one behind the other: 3230 a tile for both chains, against 2580 if the tensor cores never waited. Measured, 32
 // query and 8 KV heads: 32768 tokens, d_v 128 7.7 ms (1140 TFLOP/s, under the power cap); 8192 tokens 470 us (1170); d_v 64
-// 429 us (960). A piece takes about 7000 cycles besides its tiles (first reference, the last PV, an epilogue of 4000): 32
-// prompts of 512 tokens 135 us, 8 prompts of 64 to 2048 tokens 111.
+// 429 us (960). A piece takes about 7000 cycles besides its tiles (its first loads and reference, the last PV, the epilogue):
+// 32 prompts of 512 tokens at d_v 128 135 us, 8 prompts of 64 to 2048 tokens at d_v 64 111.
 // Tried and not kept: a polynomial for every second to eighth exponential (no faster at any share: the chain's latency is
 // what counts); leaving out the keys of a diagonal tile that a chain does not see (PV alone, by predicates: those 8 prompts
 // 117 -> 123 us; the exponentials too, as a second body for at most 64 keys: 120); S in two halves of 64 keys so that the
